@@ -9,7 +9,7 @@ Four operators make up one step of a serving program over such a cache:
   attend   the rows' attention over their requests' pages                              ops.attend_paged_kv4
 
 KV4: groups of 32 values.  m = the value of largest magnitude (the positive one when m and -m both occur),
-d = FP16(BF16(m / -8)) with |d| <= 8160, id = F32(1 / d), code = clamp(round_half_even(F32(x id)), -8, 7) + 8, value
+d = FP16(BF16(m / -8)) with |d| <= 2720, id = F32(1 / d), code = clamp(round_half_even(F32(x id)), -8, 7) + 8, value
 (code - 8) d; the codes lie two to a byte in the order of the values, low nibble first.  The planes are
 [kv_head][slot][head_dim / 2] bytes and [kv_head][slot][head_dim / 32] FP16 scales.
 """
@@ -248,7 +248,7 @@ def _quantised(x):
     """The values the cells of x stand for."""
     g = x.unflatten(-1, (-1, 32))
     top, low = g.amax(-1, keepdim=True), g.amin(-1, keepdim=True)
-    d = (torch.where(top >= -low, top, low) / -8.0).to(torch.bfloat16).float().clamp(-8160.0, 8160.0).to(torch.float16).float()
+    d = (torch.where(top >= -low, top, low) / -8.0).to(torch.bfloat16).float().clamp(-2720.0, 2720.0).to(torch.float16).float()
     inv = torch.where(d != 0, 1.0 / d, torch.zeros_like(d))
     return ((g * inv).round().clamp(-8, 7) * d).flatten(-2)
 
