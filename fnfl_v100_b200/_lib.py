@@ -12,7 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("FNB200_LIB") or os.path.join(HERE, "libfnb200.so")   # FNB200_LIB: load another build
 
 OK, REJECTED, LAUNCH_FAILED = 0, 1, 2
-ERR_TOKEN, ERR_SLOT, ERR_TIMEOUT = 1, 2, 4
+ERR_TOKEN, ERR_SLOT, ERR_TIMEOUT, ERR_PAGES = 1, 2, 4, 8
 
 
 class RopeKvArgs(C.Structure):
@@ -54,6 +54,25 @@ class AttendArgs(C.Structure):
                 ("n_q_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("scale", C.c_float)]
 
 
+class PageTablesArgs(C.Structure):
+    """fnb_page_tables_args"""
+    _fields_ = [("n_old", C.c_void_p), ("n_new", C.c_void_p), ("free_pages", C.c_void_p), ("free_head", C.c_void_p),
+                ("table", C.c_void_p), ("n_cells", C.c_void_p), ("row_start", C.c_void_p), ("slots", C.c_void_p),
+                ("pos", C.c_void_p), ("free_head_out", C.c_void_p), ("err", C.c_void_p), ("rows", C.c_int64),
+                ("n_free", C.c_int64), ("n_req", C.c_int32), ("max_pages", C.c_int32), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32)]
+
+
+class AttendPagedArgs(C.Structure):
+    """fnb_attend_paged_args"""
+    _fields_ = [("q", C.c_void_p), ("gate", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+                ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("table", C.c_void_p), ("n_cells", C.c_void_p),
+                ("row_start", C.c_void_p), ("out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("err", C.c_void_p), ("cache_slots", C.c_int64), ("rows", C.c_int32), ("n_req", C.c_int32),
+                ("max_pages", C.c_int32), ("page_size", C.c_int32), ("max_rows", C.c_int32), ("n_q_heads", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("scale", C.c_float)]
+
+
 class GgufTensor(C.Structure):
     """fnb_gguf_tensor"""
     _fields_ = [("ne", C.c_int64 * 4), ("offset", C.c_int64), ("row_bytes", C.c_int64), ("n_rows", C.c_int64),
@@ -83,6 +102,11 @@ SIGNATURES = {
     "fnb_rms_norm_act": (_I32, [_P, _P, _F, _P, _P, _P, _I64, _I32, _P, _P]),
     "fnb_rope_neox_q8_0_append": (_I32, [C.POINTER(RopeKvArgs), _P]),
     "fnb_rope_neox_kv8_append": (_I32, [C.POINTER(RopeKv8Args), _P]),
+    "fnb_rope_neox_kv4_append": (_I32, [C.POINTER(RopeKv8Args), _P]),
+    "fnb_page_tables": (_I32, [C.POINTER(PageTablesArgs), _P]),
+    "fnb_kv4_read_f32": (_I32, [C.POINTER(KvReadArgs), _P]),
+    "fnb_attend_paged_workspace_bytes": (C.c_size_t, [C.POINTER(AttendPagedArgs)]),
+    "fnb_attend_paged_kv4": (_I32, [C.POINTER(AttendPagedArgs), _P]),
     "fnb_rope_theta_scale": (_F, [_F, _I32]),
     "fnb_get_rows_q4_k": (_I32, [_P, _I64, _P, _P, _P, _I64, _I32, _P]),
     "fnb_get_rows_rms_norm_q4_k": (_I32, [_P, _I64, _P, _P, _F, _P, _P, _P, _I64, _I32, _P]),

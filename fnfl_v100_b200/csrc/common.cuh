@@ -262,5 +262,6 @@ bool expert_down_prepare_device();
 bool expert_gate_up_prepare_device();
 bool expert_down_iq4nl_prepare_device();
 bool attend_prepare_device();
+bool attend_paged_prepare_device();
 
 }  // namespace fnb

@@ -1,5 +1,5 @@
 // Per-head RMSNorm (optional) -> NeoX partial-rotary RoPE -> Q written back in F32, K and V quantised and
-// appended to the 8-bit KV cache at the token's slot.  One launch does what the CPU graph does in five ops.
+// appended to the 8-bit or 4-bit KV cache at the token's slot.  One launch does what the CPU graph does in five ops.
 //
 // HBM-bound and copy-like: per token (16 Q heads, 2 KV heads of 256) 20 KiB are read, 16 KiB of Q written
 // and 1088 bytes of cache cells written; arithmetic is a handful of flops per value plus 32 sin/cos per token.
@@ -149,6 +149,27 @@ __device__ __forceinline__ void put_kv8(const row_regs<EPL> & r, uint8_t * codes
     if (lane % G == 0) scales[lane / G] = sb;
 }
 
+// one head row -> its KV4 cell: a lane's EPL codes are EPL / 2 consecutive bytes, a group's scale leaves from its first lane
+template <int EPL>
+__device__ __forceinline__ void put_kv4(const row_regs<EPL> & r, uint8_t * codes, uint16_t * scales, int lane) {
+    constexpr int G = 32 / EPL;  // lanes per group
+    uint32_t key = 0;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) key = max(key, kv4_key(r.v[e]));
+    const kv4_rule rule(group_max_key<G>(key));
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) w |= kv4_rule::code(r.v[e], rule.id) << (4 * e);
+    if constexpr (EPL == 8) {
+        st_stream(reinterpret_cast<uint32_t *>(codes) + lane, w);
+    } else if constexpr (EPL == 4) {
+        reinterpret_cast<uint16_t *>(codes)[lane] = uint16_t(w);
+    } else {
+        codes[lane] = uint8_t(w);
+    }
+    if (lane % G == 0) scales[lane / G] = rule.db;
+}
+
 using kernel_args = rope_kernel_args;
 
 constexpr int kMaxWarps = 16;
@@ -166,10 +187,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32) rope_kv_kernel(const kernel_ar
     for (int64_t t = blockIdx.x; t < a.rows; t += gridDim.x) {
         const int32_t p = __ldg(a.pos + t);
         const int64_t slot = a.slots != nullptr ? int64_t(__ldg(a.slots + t)) : int64_t(p);
-        if (slot < 0 || slot >= a.cache_slots) {  // uniform over the CTA
-            if (threadIdx.x == 0 && a.err != nullptr) atomicOr(a.err, FNB_ERR_SLOT);
-            continue;
-        }
+        if (!rope_slot_ok<F>(slot, a.cache_slots, a.err, threadIdx.x == 0)) continue;  // uniform over the CTA
         // this warp's first two rows are requested before the angles are computed
         row_regs<EPL> r[2];
         const float * src[2];
@@ -222,6 +240,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32) rope_kv_kernel(const kernel_ar
                     if (half > 0) rope<EPL>(r[j], s_cs, half, lane);
                     if (a.k_f32 != nullptr) store_row<EPL>(r[j], a.k_f32 + (t * a.n_kv + kvh) * HD, lane);
                 }
+                if constexpr (F == kv_fmt::kv4) {
+                    const int64_t cell = int64_t(kvh) * a.cache_slots + slot;
+                    put_kv4<EPL>(r[j], (is_k ? a.k_cache : a.v_cache) + cell * (HD / 2),
+                                 (is_k ? a.k_scale : a.v_scale) + cell * EPL, lane);
+                    continue;
+                }
                 const int64_t cell = slot * a.n_kv + kvh;
                 if (F == kv_fmt::q8_0) {
                     uint8_t * dst = (is_k ? a.k_cache : a.v_cache) + cell * (EPL * 34);
@@ -256,6 +280,7 @@ int32_t launch(const fnb_rope_kv_args * p, uint16_t * k_scale, uint16_t * v_scal
         }
         if (F == kv_fmt::kv8 && (!ok_ptr(k_scale, 2) || !ok_ptr(v_scale, 2))) return FNB_REJECTED;
         if (F == kv_fmt::kv8 && hd < 64) return FNB_REJECTED;
+        if (F == kv_fmt::kv4 && (!ok_ptr(k_scale, 16) || !ok_ptr(v_scale, 16))) return FNB_REJECTED;
     }
     if (!(p->eps >= 0.0f) || !(p->theta_scale > 0.0f)) return FNB_REJECTED;
 
@@ -293,6 +318,11 @@ extern "C" int32_t fnb_rope_neox_q8_0_append(const fnb_rope_kv_args * args, void
 extern "C" int32_t fnb_rope_neox_kv8_append(const fnb_rope_kv8_args * args, void * stream) {
     if (args == nullptr) return FNB_REJECTED;
     return fnb::launch<fnb::kv_fmt::kv8>(&args->base, args->k_scale, args->v_scale, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int32_t fnb_rope_neox_kv4_append(const fnb_rope_kv8_args * args, void * stream) {
+    if (args == nullptr) return FNB_REJECTED;
+    return fnb::launch<fnb::kv_fmt::kv4>(&args->base, args->k_scale, args->v_scale, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" float fnb_rope_theta_scale(float freq_base, int32_t n_rot) {

@@ -4,10 +4,11 @@
 #pragma once
 
 #include "common.cuh"
+#include "kv4.cuh"
 
 namespace fnb {
 
-enum class kv_fmt { q8_0, kv8 };
+enum class kv_fmt { q8_0, kv8, kv4 };
 
 struct rope_kernel_args {
     const float *q, *k, *v;
@@ -32,5 +33,14 @@ __host__ __device__ __forceinline__ int rope_plane_of_pair(int i) {
 // Enqueues the pipelined kernel when the shape suits it and returns true; returns false (nothing enqueued) when
 // the caller should use the row-per-warp kernel instead.
 bool rope_kv_pipe_try_launch(const rope_kernel_args & a, int head_dim, kv_fmt fmt, cudaStream_t s);
+
+// Whether a token's slot is one to write.  A bad one is flagged, except that the paged KV4 cache's slot maps mark the
+// padding rows of a launch with -1: those are passed over in silence.
+template <kv_fmt F>
+__device__ __forceinline__ bool rope_slot_ok(int64_t slot, int64_t cache_slots, uint32_t * err, bool reports) {
+    const bool good = slot >= 0 && slot < cache_slots;
+    if (!good && reports && err != nullptr && !(F == kv_fmt::kv4 && slot == -1)) atomicOr(err, FNB_ERR_SLOT);
+    return good;
+}
 
 }  // namespace fnb

@@ -23,6 +23,7 @@
 //
 // All barrier waits are bounded.  One persistent CTA per SM.
 #include <atomic>
+#include <type_traits>
 
 #include "bulk_pipe.cuh"
 #include "exact_math.cuh"
@@ -192,9 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) rope_kv_pipe_kernel(const rope_ke
                     for (int c = 0; c < 32; ++c) theta = __fmul_rn(theta, a.theta_scale);
                 }
                 if (lane == 0) {
-                    const bool good = c_of[j] >= 0 && c_of[j] < a.cache_slots;
-                    if (!good && a.err != nullptr) atomicOr(a.err, FNB_ERR_SLOT);
-                    cell_of[s * tt + tk] = good ? int32_t(c_of[j]) : -1;
+                    cell_of[s * tt + tk] = rope_slot_ok<F>(c_of[j], a.cache_slots, a.err, true) ? int32_t(c_of[j]) : -1;
                 }
             }
             __syncwarp();
@@ -292,6 +291,34 @@ __global__ void __launch_bounds__(kThreads, 1) rope_kv_pipe_kernel(const rope_ke
                 for (int j = 0; j < NJ; ++j) st_stream(dst + 8 * j + sub, x[j]);
             }
             uint8_t * cache = kind == 1 ? a.k_cache : a.v_cache;
+            if constexpr (F == kv_fmt::kv4) {
+                // head-major planes.  Lane `sub` owns group `sub`: one rule per group, its 1 / d handed round by shuffle.
+                // A lane's four codes of a group are sixteen bits; the row's cell is put together in shared memory, and
+                // the row's eight lanes store it as 16, 8 or 4 bytes each, its scales leaving from the first of them.
+                uint32_t key[NJ];
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) key[j] = group_max_key<8>(kv4_key4(x[j]));
+                uint32_t own_key = key[0];
+#pragma unroll
+                for (int j = 1; j < NJ; ++j) own_key = sub == j ? key[j] : own_key;
+                const kv4_rule own(own_key);
+                uint16_t * s16 = reinterpret_cast<uint16_t *>(my_slot);
+                if (sub < NJ) s16[NJ * 8 + sub] = own.db;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    s16[8 * j + sub] = uint16_t(kv4_rule::code4(x[j], __shfl_sync(kFull, own.id, (lane & ~7) | j)));
+                }
+                __syncwarp();
+                if (is_kv) {
+                    using vec = std::conditional_t<HD == 256, uint4, std::conditional_t<HD == 128, uint2, uint32_t>>;
+                    const int64_t c = int64_t(hh) * a.cache_slots + cell;
+                    st_stream(reinterpret_cast<vec *>(cache + c * (HD / 2)) + sub, reinterpret_cast<const vec *>(my_slot)[sub]);
+                    uint16_t * scl = (kind == 1 ? a.k_scale : a.v_scale) + c * NJ;
+                    if (sub == 0) st_stream(reinterpret_cast<vec *>(scl), reinterpret_cast<const vec *>(my_slot)[8]);
+                }
+                __syncwarp();
+                continue;
+            }
             const int64_t c = int64_t(cell) * n_kv + hh;
             float am[NJ];
 #pragma unroll
@@ -415,6 +442,14 @@ bool launch_one(const rope_kernel_args & a, cudaStream_t s) {
 
 bool rope_kv_pipe_try_launch(const rope_kernel_args & a, int head_dim, kv_fmt fmt, cudaStream_t s) {
     const bool q8 = fmt == kv_fmt::q8_0;
+    if (fmt == kv_fmt::kv4) {
+        switch (head_dim) {
+            case 256: return launch_one<256, kv_fmt::kv4>(a, s);
+            case 128: return launch_one<128, kv_fmt::kv4>(a, s);
+            case 64: return launch_one<64, kv_fmt::kv4>(a, s);
+            default: return false;
+        }
+    }
     switch (head_dim) {
         case 256: return q8 ? launch_one<256, kv_fmt::q8_0>(a, s) : launch_one<256, kv_fmt::kv8>(a, s);
         case 128: return q8 ? launch_one<128, kv_fmt::q8_0>(a, s) : launch_one<128, kv_fmt::kv8>(a, s);
@@ -426,7 +461,9 @@ bool rope_kv_pipe_try_launch(const rope_kernel_args & a, int head_dim, kv_fmt fm
 bool rope_prepare_device() {
     return ensure_configured<256, kv_fmt::q8_0>() && ensure_configured<256, kv_fmt::kv8>() &&
            ensure_configured<128, kv_fmt::q8_0>() && ensure_configured<128, kv_fmt::kv8>() &&
-           ensure_configured<64, kv_fmt::q8_0>() && ensure_configured<64, kv_fmt::kv8>();
+           ensure_configured<64, kv_fmt::q8_0>() && ensure_configured<64, kv_fmt::kv8>() &&
+           ensure_configured<256, kv_fmt::kv4>() && ensure_configured<128, kv_fmt::kv4>() &&
+           ensure_configured<64, kv_fmt::kv4>();
 }
 
 }  // namespace fnb

@@ -9,13 +9,14 @@ is no CPU or eager fallback.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
 from . import _lib
 
 Q8_0_BLOCK, Q8_1_BLOCK, Q4_K_BLOCK, IQ3_XXS_BLOCK = 34, 36, 144, 98
-ERR_TOKEN, ERR_SLOT, ERR_TIMEOUT = _lib.ERR_TOKEN, _lib.ERR_SLOT, _lib.ERR_TIMEOUT
+ERR_TOKEN, ERR_SLOT, ERR_TIMEOUT, ERR_PAGES = _lib.ERR_TOKEN, _lib.ERR_SLOT, _lib.ERR_TIMEOUT, _lib.ERR_PAGES
 
 _TABLE_BLOCK = {"q4_k": (256, Q4_K_BLOCK), "iq3_xxs": (256, IQ3_XXS_BLOCK), "q8_0": (32, Q8_0_BLOCK)}
 
@@ -215,7 +216,11 @@ def theta_scale(freq_base: float, n_rot: int) -> float:
 
 
 def new_kv_cache(cache_slots: int, n_kv_heads: int, head_dim: int, device, fmt: str = "q8_0"):
-    """Zeroed cache planes.  q8_0: uint8 [slots][n_kv][head_dim/32*34]; kv8: (codes int8, scales fp16-bits int16)."""
+    """Zeroed cache planes.  q8_0: uint8 [slots][n_kv][head_dim/32*34]; kv8: (codes int8, scales fp16-bits int16);
+    kv4: (codes uint8 [n_kv][slots][head_dim/2], scales fp16-bits int16 [n_kv][slots][head_dim/32]), head-major."""
+    if fmt == "kv4":
+        return (torch.zeros((n_kv_heads, cache_slots, head_dim // 2), dtype=torch.uint8, device=device),
+                torch.zeros((n_kv_heads, cache_slots, head_dim // 32), dtype=torch.int16, device=device))
     if fmt == "q8_0":
         return torch.zeros((cache_slots, n_kv_heads, head_dim // 32 * Q8_0_BLOCK), dtype=torch.uint8, device=device)
     codes = torch.zeros((cache_slots, n_kv_heads, head_dim), dtype=torch.int8, device=device)
@@ -275,6 +280,142 @@ def rope_neox_kv8_append(q, k, v, pos, *, n_rot: int, theta_scale: float, k_cach
     a = _lib.RopeKv8Args(base, _ptr(k_scale).value, _ptr(v_scale).value)
     _check(_lib.lib().fnb_rope_neox_kv8_append(C.byref(a), _stream()), "rope_neox_kv8_append")
     return q_out
+
+
+# ---- the paged 4-bit cache ------------------------------------------------------------------------------------
+
+class PageTables(NamedTuple):
+    """What page_tables leaves for the step's append and attention (int32 device tensors)."""
+    slots: torch.Tensor      # [rows] cache slot of each row, -1 behind the last
+    pos: torch.Tensor        # [rows] its position within its request, -1 behind the last
+    row_start: torch.Tensor  # [n_req + 1]
+    n_cells: torch.Tensor    # [n_req]
+    free_head: torch.Tensor  # [1]
+
+
+def _out_i32(t: torch.Tensor | None, n: int, device, name: str) -> torch.Tensor:
+    if t is None:
+        return torch.empty(n, dtype=torch.int32, device=device)
+    _numel(_dev(t, torch.int32, name), n, name)
+    return t
+
+
+def page_tables(table: torch.Tensor, n_old: torch.Tensor, n_new: torch.Tensor, free_pages: torch.Tensor, *, page_size: int,
+                n_pages: int, rows: int, free_head: torch.Tensor | None = None, slots: torch.Tensor | None = None,
+                pos: torch.Tensor | None = None, row_start: torch.Tensor | None = None, n_cells: torch.Tensor | None = None,
+                free_head_out: torch.Tensor | None = None, err: torch.Tensor | None = None) -> PageTables:
+    """One step's block tables, slot map and row positions from the requests' lengths, on the device: `table`
+    [n_req][max_pages] (int32) is extended in place by the pages request r needs for its n_new[r] rows on top of n_old[r]
+    cells, taken off `free_pages` from index free_head on.  `rows` is the step's row capacity; rows behind the last request's
+    get slot -1.  n_cells may be n_old and free_head_out may be free_head.  ERR_PAGES in `err` where a request does not fit."""
+    _dev(table, torch.int32, "table")
+    if table.dim() != 2:
+        raise ValueError("table: expected [n_req][max_pages]")
+    n_req, max_pages = table.shape
+    for name, t in (("n_old", n_old), ("n_new", n_new)):
+        _numel(_dev(t, torch.int32, name), n_req, name)
+    _dev(free_pages, torch.int32, "free_pages")
+    if free_head is not None:
+        _numel(_dev(free_head, torch.int32, "free_head"), 1, "free_head")
+    d = table.device
+    with torch.cuda.device(_same_device(table, n_old, n_new, free_pages, free_head, slots, pos, row_start, n_cells, free_head_out, _err(err))):
+        o = PageTables(_out_i32(slots, rows, d, "slots"), _out_i32(pos, rows, d, "pos"), _out_i32(row_start, n_req + 1, d, "row_start"),
+                       _out_i32(n_cells, n_req, d, "n_cells"), _out_i32(free_head_out, 1, d, "free_head_out"))
+        a = _lib.PageTablesArgs(n_old.data_ptr(), n_new.data_ptr(), free_pages.data_ptr(), _ptr(free_head).value, table.data_ptr(),
+                                o.n_cells.data_ptr(), o.row_start.data_ptr(), o.slots.data_ptr(), o.pos.data_ptr(),
+                                o.free_head.data_ptr(), _ptr(err).value, rows, free_pages.numel(), n_req, max_pages, n_pages, page_size)
+        _check(_lib.lib().fnb_page_tables(C.byref(a), _stream()), "page_tables")
+    return o
+
+
+def _kv4_planes(codes: torch.Tensor, scale: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """(n_kv, slots, head_dim) of a KV4 plane from new_kv_cache(fmt="kv4")."""
+    _dev(codes, torch.uint8, name + "_cache")
+    _dev(scale, torch.int16, name + "_scale")
+    if codes.dim() != 3 or tuple(scale.shape) != (codes.shape[0], codes.shape[1], codes.shape[2] // 16):
+        raise ValueError("%s_cache / %s_scale: expected the planes of new_kv_cache(fmt=\"kv4\")" % (name, name))
+    return codes.shape[0], codes.shape[1], codes.shape[2] * 2
+
+
+def rope_neox_kv4_append(q, k, v, pos, *, n_rot: int, theta_scale: float, k_cache, v_cache, k_scale, v_scale,
+                         slots=None, q_norm_w=None, k_norm_w=None, eps: float = 1e-6, q_out=None, k_f32=None,
+                         err=None, planes=None):
+    """The norm + RoPE + append step into KV4 planes (new_kv_cache(fmt="kv4")): groups of 32 values as 4-bit codes and an
+    FP16 scale.  A slot of -1 is a row of padding, for which nothing is written.  Returns q_out."""
+    n_kv, n_slots, hd = _kv4_planes(k_cache, k_scale, "k")
+    if _kv4_planes(v_cache, v_scale, "v") != (n_kv, n_slots, hd) or tuple(k.shape[1:]) != (n_kv, hd):
+        raise ValueError("k_cache / v_cache: expected the planes of new_kv_cache for these heads")
+    if q_out is None:
+        q_out = torch.empty_like(q)
+    _numel(_dev(q_out, torch.float32, "q_out"), q.numel(), "q_out")
+    for name, t, n in (("q_norm_w", q_norm_w, hd), ("k_norm_w", k_norm_w, hd), ("k_f32", k_f32, k.numel())):
+        if t is not None:
+            _numel(_dev(t, torch.float32, name), n, name)
+    if slots is not None:
+        _dev(slots, torch.int32, "slots")
+    base = _rope_args(q, k, v, pos, slots, q_norm_w, k_norm_w, q_out, k_cache, v_cache, k_f32, _err(err), n_rot, theta_scale, eps, planes)
+    base.cache_slots = n_slots
+    a = _lib.RopeKv8Args(base, k_scale.data_ptr(), v_scale.data_ptr())
+    with torch.cuda.device(_same_device(q, k, v, pos, slots, q_norm_w, k_norm_w, q_out, k_cache, v_cache, k_scale, v_scale, k_f32, err, planes)):
+        _check(_lib.lib().fnb_rope_neox_kv4_append(C.byref(a), _stream()), "rope_neox_kv4_append")
+    return q_out
+
+
+def kv4_read_f32(cache: torch.Tensor, scale: torch.Tensor, *, cells: torch.Tensor | None = None, cell0: int = 0,
+                 rows: int | None = None, out: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows of a KV4 plane widened to F32: out [rows][n_kv][head_dim] = the values of slots cells[t] (int32), or cell0 + t."""
+    n_kv, slots, hd = _kv4_planes(cache, scale, "kv")
+    if cells is not None:
+        rows = _dev(cells, torch.int32, "cells").numel()
+    elif rows is None:
+        rows = slots - cell0
+    with torch.cuda.device(_same_device(cache, scale, cells, out, _err(err))):
+        if out is None:
+            out = torch.empty((rows, n_kv, hd), dtype=torch.float32, device=cache.device)
+        _numel(_dev(out, torch.float32, "out"), rows * n_kv * hd, "out")
+        a = _lib.KvReadArgs(cache.data_ptr(), scale.data_ptr(), _ptr(cells).value, out.data_ptr(), _ptr(err).value, rows, slots, cell0, n_kv, hd)
+        _check(_lib.lib().fnb_kv4_read_f32(C.byref(a), _stream()), "kv4_read_f32")
+    return out
+
+
+def attend_paged_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                     table: torch.Tensor, n_cells: torch.Tensor, *, page_size: int, row_start: torch.Tensor | None = None,
+                     max_rows: int = 1, scale: float | None = None, gate: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of q [rows][n_q][hd] over the paged KV4 cache: request r's rows are row_start[r] .. row_start[r + 1] - 1 (None:
+    one row a request) and see its n_cells[r] cells, the pages table[r] lists, causally.  max_rows: the most rows of a request
+    (a hint).  Rows of no request are left as they were in `out`.  `workspace` (uint8) is used when it is large enough, else one
+    is allocated.  Returns out [rows][n_q][hd]."""
+    _dev(q, torch.float32, "q")
+    n_kv, slots, hd = _kv4_planes(k_cache, k_scale, "k")
+    if q.dim() != 3 or q.shape[2] != hd or _kv4_planes(v_cache, v_scale, "v") != (n_kv, slots, hd):
+        raise ValueError("q: expected [rows][n_q_heads][head_dim]; k_cache / v_cache: planes of new_kv_cache for this head_dim")
+    _dev(table, torch.int32, "table")
+    if table.dim() != 2:
+        raise ValueError("table: expected [n_req][max_pages]")
+    n_req, max_pages = table.shape
+    _numel(_dev(n_cells, torch.int32, "n_cells"), n_req, "n_cells")
+    if row_start is not None:
+        _numel(_dev(row_start, torch.int32, "row_start"), n_req + 1, "row_start")
+    if gate is not None:
+        _numel(_dev(gate, torch.float32, "gate"), q.numel(), "gate")
+    with torch.cuda.device(_same_device(q, k_cache, v_cache, k_scale, v_scale, table, n_cells, row_start, gate, out, workspace, _err(err))):
+        if out is None:
+            out = torch.empty_like(q)
+        _numel(_dev(out, torch.float32, "out"), q.numel(), "out")
+        a = _lib.AttendPagedArgs(q.data_ptr(), _ptr(gate).value, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                                 v_scale.data_ptr(), table.data_ptr(), n_cells.data_ptr(), _ptr(row_start).value, out.data_ptr(), None, 0,
+                                 _ptr(err).value, slots, q.shape[0], n_req, max_pages, page_size, max_rows, q.shape[1], n_kv, hd,
+                                 hd ** -0.5 if scale is None else float(scale))
+        need = int(_lib.lib().fnb_attend_paged_workspace_bytes(C.byref(a)))
+        if need == 0:
+            raise ValueError("attend_paged_kv4: shape outside the contract")
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _dev(workspace, torch.uint8, "workspace")
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+        _check(_lib.lib().fnb_attend_paged_kv4(C.byref(a), _stream()), "attend_paged_kv4")
+    return out
 
 
 # ---- embedding get_rows ---------------------------------------------------------------------------------------

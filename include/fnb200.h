@@ -37,6 +37,10 @@ extern "C" {
 #define FNB_ERR_TIMEOUT 4u /* a bounded in-kernel wait gave up (the reference's device waits do the same:
                               fn/kernels/qsa/attend.cu:264-281); the launch's outputs are incomplete */
 
+#define FNB_ERR_PAGES 8u   /* fnb_page_tables: a request whose rows or pages do not fit, or a page id outside the cache;
+                              fnb_attend_paged_kv4: a page id outside the cache.  No counterpart in the reference,
+                              whose cache is one dense range */
+
 #define FNB_Q8_0_BLOCK_BYTES 34
 #define FNB_Q8_1_BLOCK_BYTES 36
 #define FNB_Q4_K_BLOCK_BYTES 144
@@ -185,6 +189,60 @@ typedef struct fnb_rope_kv8_args {
 
 int32_t fnb_rope_neox_kv8_append(const fnb_rope_kv8_args * args, void * stream);
 
+/*
+ * The same step into a cache held in 4 bits (KV4).  Per group of 32 values x of a head: m = the value of largest
+ * magnitude (the positive one when m and -m both occur), d = FP16(BF16(m / -8)) with |d| <= 2720, id = 1 / d in F32,
+ * code = clamp(nearest-even(x id), -8, 7) + 8, and the value it stands for is (code - 8) d.  A group that is all zero
+ * has d = 0 and the codes 8; a group that holds an infinity or a NaN has d = NaN.  The planes are HEAD-MAJOR: k_cache /
+ * v_cache uint8 [n_kv_heads][cache_slots][head_dim / 2], two codes a byte in the order of the values, low nibble first;
+ * k_scale / v_scale FP16 [n_kv_heads][cache_slots][head_dim / 32], 16-byte aligned.  144 bytes a 256-wide cell where
+ * Q8_0 takes 272 and KV8 264.  A slot of -1 marks a row of padding: nothing is written for it and no fault is flagged
+ * (fnb_page_tables writes such slots).  Everything else as fnb_rope_neox_kv8_append.  The reference has no 4-bit cache.
+ */
+int32_t fnb_rope_neox_kv4_append(const fnb_rope_kv8_args * args, void * stream);
+
+/*
+ * Block tables, slot map and row positions of one step over a paged cache, from the requests' lengths; everything on the
+ * device, one launch.  A page is page_size consecutive slots, page id p the slots p page_size ..; table [n_req][max_pages]
+ * lists each request's pages in the order of its cells, its first ceil(n_old / page_size) entries being those it holds.
+ * Request r gets n_new[r] rows on top of its n_old[r] cells (either may be 0):
+ *   table         the pages it needs beyond those it holds, off the free list: the requests in order take free_pages
+ *                 [*free_head ..] one after another (free_head null: from the list's beginning;
+ *                 outside [0, n_free]: an empty list)
+ *   n_cells       [n_req]      n_old + n_new, or n_old for a request that was given nothing
+ *   row_start     [n_req + 1]  its rows are row_start[r] .. row_start[r + 1] - 1 (sums of n_new)
+ *   slots, pos    [rows]       each row's cache slot and position (its index within the request); -1 in both for rows
+ *                 behind the last request's, which is what a padded launch's append passes over
+ *   free_head_out (optional)   *free_head + the pages taken
+ * A request gets nothing (its rows have slots and pos -1, n_cells its old length, no page is taken) when a length is
+ * negative, when its cells would not fit into max_pages pages, when its rows end behind `rows`, or when the free list
+ * does not reach; FNB_ERR_PAGES is then set.  Once the list does not reach, later requests that need a page get nothing
+ * either.  A page id outside [0, n_pages) sets FNB_ERR_PAGES and the rows in that page have slot -1.
+ * n_cells may be n_old and free_head_out may be free_head (a captured graph's persistent state); no other two arrays may
+ * overlap.  n_req in [1, 2048]; page_size a power of two; n_pages page_size < 2^31.  No counterpart in the reference.
+ */
+typedef struct fnb_page_tables_args {
+    const int32_t * n_old;
+    const int32_t * n_new;
+    const int32_t * free_pages; /* [n_free] */
+    const int32_t * free_head;  /* [1] or null */
+    int32_t * table;
+    int32_t * n_cells;
+    int32_t * row_start;
+    int32_t * slots;
+    int32_t * pos;
+    int32_t * free_head_out; /* [1] or null */
+    uint32_t * err;
+    int64_t rows;
+    int64_t n_free;
+    int32_t n_req;
+    int32_t max_pages;
+    int32_t n_pages;
+    int32_t page_size;
+} fnb_page_tables_args;
+
+int32_t fnb_page_tables(const fnb_page_tables_args * args, void * stream);
+
 /* theta_scale = powf(freq_base, -2 / n_rot), the host-side constant of fn/kernels/qsa/attend.cu:830-832. */
 float fnb_rope_theta_scale(float freq_base, int32_t n_rot);
 
@@ -308,6 +366,13 @@ typedef struct fnb_kv_read_args {
 int32_t fnb_kv_read_f32(const fnb_kv_read_args * args, void * stream);
 
 /*
+ * The same for a KV4 plane (fnb_rope_neox_kv4_append's layout): cache the codes [n_kv_heads][cache_slots][head_dim / 2],
+ * scale the FP16 plane [n_kv_heads][cache_slots][head_dim / 32], 16-byte aligned and required.  out[t][h][:] =
+ * (code - 8) d of slot cells[t] (or cell0 + t).  A slot of -1 (padding) leaves its row untouched without a fault.
+ */
+int32_t fnb_kv4_read_f32(const fnb_kv_read_args * args, void * stream);
+
+/*
  * Decode attention over the cache the append entry points write: for each of `rows` query rows t and query head h,
  *   out[t][h] = softmax over the row's cells c of (scale q[t][h] . K[c][g]) applied to V[c][g],  g = h / (n_q_heads / n_kv_heads),
  * times sigmoid(gate[t][h]) when gate is given (the reference's output gate).  q [rows][n_q_heads][head_dim] F32 is the
@@ -378,6 +443,61 @@ int32_t fnb_attend(const fnb_attend_args * args, void * stream);
  *     workspace of their own through fnb_attend.
  */
 int32_t fnb_attend_static(const fnb_attend_args * args, void * stream);
+
+/*
+ * Attention of many requests over a paged KV4 cache, in one call: the decode (or drafted, or short prefill) rows of
+ * n_req requests, each over its own cells.
+ *   out[t][h] = softmax over the row's cells c of (scale q[t][h] . K[c][g]) applied to V[c][g],  g = h / (n_q_heads / n_kv_heads),
+ * times sigmoid(gate[t][h]) when gate is given.  q [rows][n_q_heads][head_dim] F32 is the q_out of
+ * fnb_rope_neox_kv4_append; the planes are that entry point's, K and V the values (code - 8) d of their cells.
+ * Request r holds n_cells[r] cells in the pages table[r][0 ..] lists (cell c: slot table[r][c / page_size] page_size +
+ * c % page_size), its rows are row_start[r] .. row_start[r + 1] - 1 (row_start null: one row a request), and its rows
+ * are its last cells: row i of m sees the first n_cells[r] - m + i + 1 of them (causal).  All three arrays are read on
+ * the device, so one captured graph serves every step; fnb_page_tables writes them.  A row that sees no cell gives
+ * zeros; rows that belong to no request are left as they were.  What lies in a page behind a request's last cell, or in
+ * cells a row does not see, does not touch its result, NaN included.
+ * max_rows (a hint; 0 means 1): the most rows a request has.  Requests of at most max_rows rows have their cells read
+ * once; up to 64 query rows a KV head (rows x n_q_heads / n_kv_heads) are served in one pass.
+ * F32 softmax statistics; products on the tensor cores with queries and probabilities split into two FP16 parts, cells
+ * exact: relative error (2-norm) against a 64-bit evaluation about 1e-6.  |q| below 2^64.
+ * A page id outside the cache, a length outside [0, max_pages page_size], or a row range outside [0, rows) sets
+ * FNB_ERR_PAGES; the rows of that request then mean nothing, others are unaffected.
+ * head_dim 64, 128 or 256; n_req in [1, 2048]; page_size a power of two from 16 on; cache_slots a multiple of page_size;
+ * q, gate, out, caches and scales 16-byte aligned.  out may not overlap an input.
+ * workspace: at least fnb_attend_paged_workspace_bytes(args) bytes (a function of head_dim, max_rows, the head counts
+ * and whether max_pages page_size exceeds 128, not of the lengths), 16-byte aligned; its contents need no
+ * initialisation and mean nothing afterwards.  Calls that share a workspace must not overlap on the GPU.
+ * The first call per device and shape class raises a kernel attribute (fnb_prepare_device covers it).
+ * The reference attends one dense range per call (fn/kernels/qsa/attend.h:9-23); pages have no counterpart there.
+ */
+typedef struct fnb_attend_paged_args {
+    const float * q;
+    const float * gate;
+    const void * k_cache;
+    const void * v_cache;
+    const uint16_t * k_scale;
+    const uint16_t * v_scale;
+    const int32_t * table;
+    const int32_t * n_cells;
+    const int32_t * row_start;
+    float * out;
+    void * workspace;
+    size_t workspace_bytes;
+    uint32_t * err;
+    int64_t cache_slots;
+    int32_t rows;
+    int32_t n_req;
+    int32_t max_pages;
+    int32_t page_size;
+    int32_t max_rows;
+    int32_t n_q_heads;
+    int32_t n_kv_heads;
+    int32_t head_dim;
+    float scale;
+} fnb_attend_paged_args;
+
+size_t fnb_attend_paged_workspace_bytes(const fnb_attend_paged_args * args); /* 0 for a shape outside the contract */
+int32_t fnb_attend_paged_kv4(const fnb_attend_paged_args * args, void * stream);
 
 /*
  * F32 rows to ggml Q8_K blocks (292 bytes per 256 values: F32 d, 256 int8 codes, 16 int16 sums of 16 codes), the
