@@ -29,16 +29,15 @@
 // all tiles of an item writes its rows itself; otherwise it leaves its sums, maximum and accumulators in the workspace
 // and a second launch folds an item's pieces in their order.  Results do not depend on timing.
 //
-// A CTA is eight warps.  Scores: a warp takes 16 cells for eight columns, whose query fragments it keeps in registers.
-// Maxima cross the warps through shared memory, probabilities go there in the order of the second product's fragments,
-// and there a warp takes 32 dims of all cells.  K and V tiles take turns in a ring that warp 0 feeds: per page one
-// tensor-map copy of a plane's codes, swizzled so that ldmatrix has no bank conflicts, and one bulk copy of its scales.
-// The barrier between a tile's scores and its probabilities is also the proof that the tile's K stage and the V stage
-// before it are no longer read, so the ring needs no barriers of its own for that, and no warp is set aside for the
-// copies (a ninth warp would cost the other eight a quarter of their registers: 18 warps an SM put five on a scheduler).
-#include <cuda.h>  // CUtensorMap and the type of cuTensorMapEncodeTiled (reached through cudaGetDriverEntryPoint)
-
+// A CTA is eight warps.  Scores: a warp takes 16 cells for eight columns.  Maxima cross the warps through shared memory,
+// probabilities go there in the order of the second product's fragments, and there a warp takes 32 dims of all cells.
+// Scores run a tile ahead of outputs, so one barrier a tile is enough: two K stages and three V stages, which every
+// thread fills for two tiles ahead with its share of 16-byte asynchronous copies, and each thread's wait for its own
+// copies before the barrier makes them everybody's.  Nothing else waits.  (Tensor-map copies, a page each, were tried
+// first: a page's four copies are issued one after another, by one warp that the seven others then wait for, or that
+// costs them registers as a ninth: 18 warps an SM put five on a scheduler.  61 us became XXX at 196 608 cells.)
 #include <atomic>
+#include <type_traits>
 
 #include "bulk_pipe.cuh"
 #include "kv4.cuh"
@@ -63,25 +62,26 @@ struct geo {
     static constexpr int kCodeBytes = kTileCells * HD / 2, kScaleBytes = kTileCells * kGroups * 2;
     static constexpr int kUnitBytes = kCodeBytes + kScaleBytes;
     static constexpr int kCtas = NT <= 2 ? 2 : 1;               // resident on an SM (registers)
-    static constexpr int kRing = HD == 256 ? (NT <= 2 ? 5 : 7) : (NT <= 2 ? 9 : 13);  // odd (feed_step)
+    static constexpr int kVStages = 3, kStages = 2 + kVStages;   // K's, then V's
     static constexpr uint32_t kSwz = HD == 256 ? 7u : HD == 128 ? 3u : 1u;
     // shared memory
     static constexpr int ring = 0;
-    static constexpr int prob = ring + kRing * kUnitBytes;      // uint4 [2][8 slabs][NT][32]
-    static constexpr int wmax = prob + 2 * 8 * NT * 512;        // float [2][8 warps][8]
+    static constexpr int prob = ring + kStages * kUnitBytes;    // uint4 [2][8 slabs][NT][32]
+    static constexpr bool kShareQueries = NT == 1;              // one column block: every warp has the same fragments
+    static constexpr int qfrag = prob + 2 * 8 * NT * 512;       // uint4 [kGroups][hi, lo][32]
+    static constexpr int wmax = qfrag + (kShareQueries ? kGroups * 1024 : 0);  // float [2][8 warps][8]
     static constexpr int lsum = wmax + 512;                     // float [8 warps][8]
     static constexpr int corr = lsum + 256;                     // float [2][kCols]
     static constexpr int mfin = corr + 2 * kCols * 4;           // float [kCols]
     static constexpr int red = mfin + kCols * 4;                // float4: the other cell groups' accumulators
-    static constexpr int bars = red + (kCellGroups - 1) * kGroups * 32 * kCols * 4;
-    static constexpr int scan = bars + kRing * 8;               // int64 [8]: sums; then the start of this CTA's piece
-    static constexpr int feed = scan + 12 * 8;                  // the feeder's walk
-    static constexpr int total = feed + 64 + 1024;              // + slack to align the base to 1024 bytes
+    static constexpr int scan = red + (kCellGroups - 1) * kGroups * 32 * kCols * 4;  // int64 [8]: sums; the piece's start
+    static constexpr int total = scan + 10 * 8 + 1024;          // + slack to align the base to 1024 bytes
     static_assert(total * kCtas + 1024 * kCtas <= 233472, "shared memory of an SM");
 };
 
 struct paged_params {
     const float *q, *gate;
+    const uint8_t *k_cache, *v_cache;
     const uint16_t *k_scale, *v_scale;
     const int32_t *table, *n_cells, *row_start;
     float * out;
@@ -145,23 +145,18 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void tensor_g2s(void * dst, const CUtensorMap * map, int y, int z, uint64_t * bar, uint64_t policy) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(
-            smem_u32(dst)),
-        "l"(map), "r"(0), "r"(y), "r"(z), "r"(smem_u32(bar)), "l"(policy)
-        : "memory");
-}
-// bounded; once a wait has run out, the CTA's others return at their next look and it runs to its end on what it has
-__device__ __forceinline__ bool ring_wait(uint64_t * bar, uint32_t parity, volatile uint32_t * gave_up, uint32_t * err) {
-    for (uint32_t i = 0; i < kPrimarySpinLimit; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 63u) == 63u && *gave_up != 0) return false;
+// BYTES from global to shared memory behind the thread's back, or as many zeros
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void * src, bool some) {
+    if constexpr (BYTES == 16) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(some ? 16 : 0) : "memory");
+    } else {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(some ? BYTES : 0), "n"(BYTES) : "memory");
     }
-    *gave_up = 1;
-    if (err != nullptr) atomicOr(err, FNB_ERR_TIMEOUT);
-    return false;
 }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 // A request as every thread that walks the units sees it.
 struct request {
@@ -232,104 +227,97 @@ struct fold_head {
     int32_t fold, from, to, r, h, blk;
 };
 
-// ---- the ring's feeder: warp 0's walk, kept in shared memory (its registers are the query fragments') ----------------
-// The ring's order is K0 | K1 V0 | K2 V1 | ... | V(n - 1), the order in which stages fall free: scores run a tile ahead of
-// outputs.  Step j issues K(j) from the lower half-warp and V(j - 1) from the upper one, a lane a page.
-struct feeder {
-    int r, h, blk, tile;
-    int n, m, tiles, blocks;   // the walk's request
-    uint32_t step, tiles_all;  // tiles of the piece
-    int stage;                 // the next unit's
-    int v_h, v_live;           // head and pages of the tile whose V is next
-};
-// where tile j's K and V are, of n tiles
-__device__ __forceinline__ uint32_t unit_of_k(uint32_t j) { return j == 0 ? 0 : 2 * j - 1; }
-__device__ __forceinline__ uint32_t unit_of_v(uint32_t j, uint32_t n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; }
-
-// One step, if there is one.  Warp 0, all lanes.  `id`: this (lower) lane's page of the K tile, fetched a step ahead;
-// `slot`: this (upper) lane's first slot of the V tile.
+// ---- the copies -------------------------------------------------------------------------------------------------------
+// Step s of a piece brings tile s's K and tile s - 1's V.  A warp copies sixteen rows, which lie in one page: one page id
+// a warp and tile, fetched a step ahead, and addresses that differ by constants.  A lane copies one 16-byte chunk (a
+// group's codes) of kPass rows, and one row's scales, K's (lower half-warp) or V's.  Chunk c of a row lies at c ^ (bits
+// of the row), which keeps ldmatrix free of bank conflicts.  The walk runs two tiles ahead of the scores.
 template <int HD, int NT>
-__device__ __forceinline__ void feed_step(const paged_params & p, const CUtensorMap * map_k, const CUtensorMap * map_v, feeder * f,
-                                          uint8_t * smem, uint64_t * full, int32_t & slot, int32_t & id, uint64_t policy) {
+struct loader {
     using G = geo<HD, NT>;
-    const uint32_t j = f->step, n = f->tiles_all;
-    if (j > n) return;
-    const int lane = threadIdx.x & 31, at = lane & 15;
-    const bool upper = lane >= 16;
-    const int page = 1 << p.page_shift, box = page < kTileCells ? page : kTileCells;
-    const int base = f->tile * kTileCells, left = f->n - base, h = f->h;
-    const int k_live = j == n || left <= 0 ? 0 : min(kTileCells / box, (left + box - 1) / box);
-    const int live = upper ? f->v_live : k_live;
-    int stage = f->stage;
-    if (upper && j > 0 && j < n) stage = stage + 1 == G::kRing ? 0 : stage + 1;
-    if (!upper && at < k_live) {
-        if (id < 0 || id >= p.n_pages) {
-            if (p.err != nullptr) atomicOr(p.err, FNB_ERR_PAGES);
-            id = 0;
-        }
-        slot = int32_t((uint32_t(id) << p.page_shift) + uint32_t((base + at * box) & (page - 1)));
+    static constexpr int kCh = G::kGroups, kRows = 32 / kCh, kPass = 16 / kRows, kRow = HD / 2, kScale = kCh * 2;
+    cursor<G::kCols> c;
+    uint32_t step, tiles;  // of the piece
+    uint32_t v_stage;
+    int32_t id;            // page of the warp's rows in tile `step`
+    uint32_t cell;         // first of its rows in tile `step` - 1, counted through all heads of a plane
+    int v_left;            // that tile's cells from the warp's first row on
+    uint32_t lane_to;      // this lane's chunk of the warp's first pass within a stage
+
+    __device__ __forceinline__ static int warp_row() { return int(threadIdx.x >> 5) * 16; }
+    __device__ __forceinline__ void fetch(const paged_params & p) {
+        const int at = c.tile * kTileCells + warp_row();
+        id = at < c.x.n ? __ldg(p.table + int64_t(c.r) * p.max_pages + (at >> p.page_shift)) : 0;
     }
-    uint8_t * st = smem + G::ring + stage * G::kUnitBytes;
-    if (at == 0 && (upper ? j > 0 : j < n)) {
-        mbar_expect_tx(&full[stage], uint32_t(live) * uint32_t(box) * (HD / 2 + G::kGroups * 2));
-        mbar_arrive(&full[stage]);
+    __device__ __forceinline__ void start(const paged_params & p, const cursor<G::kCols> & from, uint32_t n) {
+        c = from, step = 0, tiles = n, v_stage = G::kVStages - 1, v_left = 0, cell = 0;
+        fetch(p);
+        const uint32_t lane = threadIdx.x & 31, row = uint32_t(warp_row()) + lane / kCh;
+        lane_to = row * kRow + (((lane % kCh) ^ ((row * kRow >> 7) & G::kSwz)) << 4);
     }
-    __syncwarp();
-    if (at < live) {
-        const int head = upper ? f->v_h : h;
-        tensor_g2s(st + at * box * (HD / 2), upper ? map_v : map_k, slot, head, &full[stage], policy);
-        const uint16_t * scale = (upper ? p.v_scale : p.k_scale) + (int64_t(head) * p.cache_slots + slot) * G::kGroups;
-        bulk_g2s(st + G::kCodeBytes + at * box * G::kGroups * 2, scale, uint32_t(box) * G::kGroups * 2, &full[stage], policy);
-    }
-    slot = __shfl_sync(kFull, slot, at);
-    __syncwarp();
-    if (lane == 0) {
-        f->v_h = h, f->v_live = k_live, f->step = j + 1;
-        const int next = f->stage + (j == 0 || j == n ? 1 : 2);
-        f->stage = next >= G::kRing ? next - G::kRing : next;
-    }
-    if (j + 1 < n) {
-        cursor<G::kCols> c;
-        c.r = f->r, c.h = h, c.blk = f->blk, c.tile = f->tile + 1;
-        c.x.n = f->n, c.x.m = f->m, c.x.tiles = f->tiles, c.x.blocks = f->blocks;
-        if (c.tile >= c.x.tiles) {
-            c.next_item(p);
-            __syncwarp();
-            if (lane == 0) {
-                f->r = c.r, f->h = c.h, f->blk = c.blk;
-                f->n = c.x.n, f->m = c.x.m, f->tiles = c.x.tiles, f->blocks = c.x.blocks;
+    // `left` (at most sixteen count) of the rows at cell `first` into the stage at `st`
+    __device__ __forceinline__ void rows(const uint8_t * plane, uint32_t first, int left, uint32_t st) const {
+        const uint32_t lane = threadIdx.x & 31;
+        const uint8_t * src = plane + uint64_t(first) * kRow + lane * 16;
+        const uint32_t to = st + lane_to;
+        // a 256-wide cell: four rows a pass, so every second pass has the other half of the eight row patterns
+        if (left >= 16) {
+#pragma unroll
+            for (int i = 0; i < kPass; ++i) copy_async<16>((to + i * kRows * kRow) ^ (kRows == 4 && (i & 1) ? 64u : 0u), src + i * kRows * kRow, true);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPass; ++i) {
+                copy_async<16>((to + i * kRows * kRow) ^ (kRows == 4 && (i & 1) ? 64u : 0u), src + i * kRows * kRow, int(lane / kCh) + i * kRows < left);
             }
         }
-        __syncwarp();
-        if (lane == 0) f->tile = c.tile;
-        const int cell = c.tile * kTileCells + at * box;
-        id = !upper && at * box < kTileCells && cell < c.x.n ? __ldg(p.table + int64_t(c.r) * p.max_pages + (cell >> p.page_shift)) : -1;
     }
-    __syncwarp();
-}
+    __device__ __forceinline__ void next(const paged_params & p, uint32_t ring) {
+        if (step > tiles) return;
+        const uint32_t lane = threadIdx.x & 31;
+        const bool k_too = step < tiles, v_too = step > 0;
+        const uint32_t k_st = ring + (step & 1) * G::kUnitBytes, v_st = ring + (2 + v_stage) * G::kUnitBytes;
+        const uint32_t v_cell = cell;
+        const int old_left = v_left;
+        if (v_too) rows(p.v_cache, v_cell, old_left, v_st);
+        if (k_too) {
+            const int base = c.tile * kTileCells + warp_row();
+            v_left = c.x.n - base;
+            if (uint32_t(id) >= uint32_t(p.n_pages)) {
+                if (lane == 0 && p.err != nullptr) atomicOr(p.err, FNB_ERR_PAGES);
+                id = 0;
+            }
+            cell = uint32_t(c.h) * uint32_t(p.cache_slots) + (uint32_t(id) << p.page_shift) + (uint32_t(base) & ((1u << p.page_shift) - 1));
+            rows(p.k_cache, cell, v_left, k_st);
+        }
+        const bool lower = lane < 16;
+        if (lower ? k_too : v_too) {
+            const uint32_t at = (lower ? cell : v_cell) + (lane & 15);
+            copy_async<kScale>((lower ? k_st : v_st) + G::kCodeBytes + uint32_t(warp_row() + (lane & 15)) * kScale,
+                               (lower ? p.k_scale : p.v_scale) + uint64_t(at) * kCh, int(lane & 15) < (lower ? v_left : old_left));
+        }
+        copies_commit();
+        if (step + 1 < tiles) {
+            if (++c.tile >= c.x.tiles) c.next_item(p);
+            fetch(p);
+        }
+        ++step;
+        v_stage = v_stage + 1 == G::kVStages ? 0 : v_stage + 1;
+    }
+};
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------
 template <int HD, int NT>
 __global__ void __launch_bounds__(kThreadsC, geo<HD, NT>::kCtas)
-attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+attend_paged_kernel(const __grid_constant__ paged_params p) {
     using G = geo<HD, NT>;
     constexpr int NB = G::kGroups;
     extern __shared__ uint8_t smem_raw[];
     uint8_t * smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (rounding the pointer itself would make every access a generic one)
-    uint64_t * full = reinterpret_cast<uint64_t *>(smem + G::bars);
-    feeder * s_feed = reinterpret_cast<feeder *>(smem + G::feed);
     int64_t * s_scan = reinterpret_cast<int64_t *>(smem + G::scan);
-    volatile uint32_t * s_misc = reinterpret_cast<volatile uint32_t *>(s_scan + 8);  // [0] start request, [1] gave up, [2] start within it
+    volatile uint32_t * s_start = reinterpret_cast<volatile uint32_t *>(s_scan + 8);  // the piece's first request, its unit there
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
 
     pdl_launch_dependents();
-    if (tid == 0) {
-        for (int s = 0; s < G::kRing; ++s) {
-            mbar_init(&full[s], 1);
-        }
-        mbar_init_fence();
-        s_misc[1] = 0;
-    }
     pdl_wait();
 
     // where this CTA's piece starts: sums of the requests' units, formed by every CTA for itself
@@ -365,8 +353,8 @@ attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap ma
         for (int j = 0; j < per; ++j) {
             const int64_t units = units_of(p, load_request<G::kCols>(p, tid * per + j, false));
             if (base + units > int64_t(u0)) {
-                s_misc[0] = uint32_t(tid * per + j);
-                s_misc[2] = u0 - uint32_t(base);
+                s_start[0] = uint32_t(tid * per + j);
+                s_start[1] = u0 - uint32_t(base);
                 break;
             }
             base += units;
@@ -378,7 +366,10 @@ attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap ma
         return;
     }
     cursor<G::kCols> c;
-    c.at(p, int(s_misc[0]), s_misc[2]);
+    c.at(p, int(s_start[0]), s_start[1]);
+    const uint32_t ring = smem_u32(smem) + G::ring;
+    loader<HD, NT> load;
+    load.start(p, c, u1 - u0);
     if (tid == kThreadsC - 1 && p.ws_head != nullptr) {
         fold_head f = {0, 0, 0, c.r, c.h, c.blk};
         if (c.tile != 0) {
@@ -387,25 +378,6 @@ attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap ma
             f.fold = int(blockIdx.x) == f.from + 1;                // a cut piece is never empty, so neither is the next
         }
         *reinterpret_cast<fold_head *>(p.ws_head + int64_t(blockIdx.x) * 8) = f;
-    }
-
-    // the ring is filled before anything else
-    const uint64_t policy = l2_evict_first_policy();
-    int32_t feed_slot = 0, feed_id = -1;  // warp 0's
-    auto feed = [&]() {
-        if (s_misc[1] == 0) feed_step<HD, NT>(p, &map_k, &map_v, s_feed, smem, full, feed_slot, feed_id, policy);
-    };
-    if (wid == 0) {
-        const int page = 1 << p.page_shift, box = page < kTileCells ? page : kTileCells;
-        const int at = lane & 15, cell = c.tile * kTileCells + at * box;
-        feed_id = lane < 16 && at * box < kTileCells && cell < c.x.n ? __ldg(p.table + int64_t(c.r) * p.max_pages + (cell >> p.page_shift)) : -1;
-        if (lane == 0) {
-            s_feed->r = c.r, s_feed->h = c.h, s_feed->blk = c.blk, s_feed->tile = c.tile;
-            s_feed->n = c.x.n, s_feed->m = c.x.m, s_feed->tiles = c.x.tiles, s_feed->blocks = c.x.blocks;
-            s_feed->step = 0, s_feed->tiles_all = u1 - u0, s_feed->stage = 0, s_feed->v_h = 0, s_feed->v_live = 0;
-        }
-        __syncwarp();
-        for (int k = 0; k <= G::kRing / 2; ++k) feed();
     }
 
     const int g = lane >> 2, t = lane & 3;
@@ -417,19 +389,15 @@ attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap ma
     float * s_corr = reinterpret_cast<float *>(smem + G::corr);
     float * s_mfin = reinterpret_cast<float *>(smem + G::mfin);
     uint4 * s_prob = reinterpret_cast<uint4 *>(smem + G::prob);
-    // ldmatrix: a lane's row of a tile and its 16-byte chunk there, which the copy's swizzle has xored with bits of the
-    // row (the same for every sixteenth row, so all addresses of a lane differ by constants)
+    uint4 * s_q = reinterpret_cast<uint4 *>(smem + G::qfrag);
+    // ldmatrix: a lane's row of a tile and its 16-byte chunk there, which the loader has xored with bits of the row
+    // (the same for every sixteenth row, so all addresses of a lane differ by constants)
     const int lrow = (lane & 7) + ((lane >> 3) & 1) * 8, lhalf = lane >> 4;
     const uint32_t swz = (uint32_t(lrow) * (HD / 2) >> 7) & G::kSwz;
     const uint32_t k_off = uint32_t(slab0 * 16 + lrow) * (HD / 2) + ((uint32_t(lhalf) ^ swz) << 4);                 // groups 0, 1
     const uint32_t v_off = uint32_t(cg * kSlabs * 16 + lhalf * 16 + lrow) * (HD / 2) + ((uint32_t(dg) ^ swz) << 4);  // slabs 0, 1
 
-    uint32_t tile_no = 0;  // tiles of the piece begun
-    auto unit_ready = [&](uint32_t unit) {
-        const uint32_t turn = unit / G::kRing, stage = unit - turn * G::kRing;
-        (void) ring_wait(&full[stage], turn & 1u, s_misc + 1, p.err);
-        return smem + G::ring + stage * G::kUnitBytes;
-    };
+    uint32_t k_stage = 0, v_stage = 0;  // of the next tile scored, of the next tile put out
     uint32_t u = u0;
     while (u < u1) {
         const int tile_first = c.tile;
@@ -438,40 +406,81 @@ attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap ma
         const int col0 = c.blk * G::kCols;
         auto row_of_col = [&](int col) { return (col0 + col) / p.group; };
 
-        // queries of column 8 nt + g: this lane's eight dims of every group, in the order of the fragments
-        uint32_t qf[NB][8];      // per group: n0n1 hi b0 b1, lo b0 b1; n2n3 hi, lo
+        // Queries of column 8 nt + g, split, in the order of the fragments: dims 8 t + {0, 4}, {1, 5}, {2, 6}, {3, 7} of a
+        // group, which are nibbles 0 .. 3 of the two halves of a cell's word.
+        uint32_t qh[NB][4];                                  // hi parts
+        uint32_t ql[G::kShareQueries ? 1 : NB][4];           // lo parts
         float sc0, sc1;
         int lim0, lim1;
         {
             const int col = nt * 8 + g, i = row_of_col(col);
             const bool on = i < c.x.m;
             const float * src = p.q + (int64_t(c.x.row0 + (on ? i : 0)) * p.n_q + c.h * p.group + (col0 + col) % p.group) * HD + 8 * t;
-            float4 v[NB][2];
-            float top = 0.0f;
+            const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto load8 = [&](int b, float4 (&v)[2]) {
+                v[0] = on ? __ldg(reinterpret_cast<const float4 *>(src + 32 * b)) : zero;
+                v[1] = on ? __ldg(reinterpret_cast<const float4 *>(src + 32 * b + 4)) : zero;
+            };
+            auto top8 = [&](const float4 (&v)[2]) {
+                return fmaxf(fmaxf(fmaxf(fabsf(v[0].x), fabsf(v[0].y)), fmaxf(fabsf(v[0].z), fabsf(v[0].w))),
+                             fmaxf(fmaxf(fabsf(v[1].x), fabsf(v[1].y)), fmaxf(fabsf(v[1].z), fabsf(v[1].w))));
+            };
+            auto split8 = [&](const float4 (&v)[2], float up, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+                split2(__fmul_rn(v[0].x, up), __fmul_rn(v[1].x, up), hi[0], lo[0]);
+                split2(__fmul_rn(v[0].y, up), __fmul_rn(v[1].y, up), hi[1], lo[1]);
+                split2(__fmul_rn(v[0].z, up), __fmul_rn(v[1].z, up), hi[2], lo[2]);
+                split2(__fmul_rn(v[0].w, up), __fmul_rn(v[1].w, up), hi[3], lo[3]);
+            };
+            // the power of two that takes the row's largest into [2^13, 2^14), and its inverse
+            auto powers = [&](float top, float & up, float & down) {
+                int e = int(__float_as_uint(top) >> 23);
+                e = e < 14 ? 14 : e > 254 ? 254 : e;
+                up = __uint_as_float(uint32_t(267 - e) << 23), down = __uint_as_float(uint32_t(e - 13) << 23);
+            };
+            float up, down;
+            if constexpr (G::kShareQueries) {
+                // a group a warp; the maxima and then the fragments cross the warps
+                float4 v[2] = {zero, zero};
+                if (wid < NB) load8(wid, v);
+                if (load.step == 0) load.next(p, ring);      // the piece's first copies, while the queries arrive
+                float top = top8(v);
+                top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+                if (t == 0) s_wmax[wid * 8 + g] = top;
+                if (load.step == 1) load.next(p, ring);
+                named_barrier<1>(kThreadsC);
+                top = 0.0f;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                v[b][0] = on ? __ldg(reinterpret_cast<const float4 *>(src + 32 * b)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                v[b][1] = on ? __ldg(reinterpret_cast<const float4 *>(src + 32 * b + 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    top = fmaxf(top, fmaxf(fmaxf(fabsf(v[b][j].x), fabsf(v[b][j].y)), fmaxf(fabsf(v[b][j].z), fabsf(v[b][j].w))));
+                for (int b = 0; b < NB; ++b) top = fmaxf(top, s_wmax[b * 8 + g]);
+                powers(top, up, down);
+                if (wid < NB) {
+                    uint32_t hi[4], lo[4];
+                    split8(v, up, hi, lo);
+                    s_q[wid * 64 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    s_q[wid * 64 + 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
-            }
-            top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-            int e = int(__float_as_uint(top) >> 23);
-            e = e < 14 ? 14 : e > 254 ? 254 : e;
-            const float up = __uint_as_float(uint32_t(267 - e) << 23), down = __uint_as_float(uint32_t(e - 13) << 23);
+                copies_wait<1>();                            // K of the piece's first tile
+                named_barrier<1>(kThreadsC);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                // dims 8 t + {0, 4}, {1, 5}, {2, 6}, {3, 7}: nibbles 0 .. 3 of the two halves of a cell's word
-                split2(__fmul_rn(v[b][0].x, up), __fmul_rn(v[b][1].x, up), qf[b][0], qf[b][2]);
-                split2(__fmul_rn(v[b][0].y, up), __fmul_rn(v[b][1].y, up), qf[b][1], qf[b][3]);
-                split2(__fmul_rn(v[b][0].z, up), __fmul_rn(v[b][1].z, up), qf[b][4], qf[b][6]);
-                split2(__fmul_rn(v[b][0].w, up), __fmul_rn(v[b][1].w, up), qf[b][5], qf[b][7]);
+                for (int b = 0; b < NB; ++b) {
+                    const uint4 v4 = s_q[b * 64 + lane];
+                    qh[b][0] = v4.x, qh[b][1] = v4.y, qh[b][2] = v4.z, qh[b][3] = v4.w;
+                }
+            } else {
+                while (load.step < 2 && load.step <= u1 - u0) load.next(p, ring);
+                float4 v[NB][2];
+                float top = 0.0f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) load8(b, v[b]);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) top = fmaxf(top, top8(v[b]));
+                top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+                powers(top, up, down);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) split8(v[b], up, qh[b], ql[G::kShareQueries ? 0 : b]);
+                copies_wait<1>();
+                named_barrier<1>(kThreadsC);
             }
             const float sc = fmaxf(p.scale_log2 * down, 0x1p-126f);
             sc0 = __shfl_sync(kFull, sc, 8 * t), sc1 = __shfl_sync(kFull, sc, 8 * t + 4);
@@ -495,8 +504,9 @@ attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap ma
         // scores of tile `it` of the item into sv, their maxima to the other warps
         auto scores = [&](int it) {
             const int base = (tile_first + it) * kTileCells;
-            uint8_t * kt = unit_ready(unit_of_k(tile_no + it));
-            const uint32_t k_addr = smem_u32(kt) + k_off;
+            const uint8_t * kt = smem + G::ring + k_stage * G::kUnitBytes;
+            const uint32_t k_addr = ring + k_stage * G::kUnitBytes + k_off;
+            k_stage ^= 1;
 #pragma unroll
             for (int s = 0; s < NT; ++s) {
                 const int row = (slab0 + s) * 16;
@@ -523,10 +533,17 @@ attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap ma
                         const uint32_t x0 = w[2 * j], x1 = w[2 * j + 1], y0 = x0 >> 8, y1 = x1 >> 8;
                         const uint32_t a0 = code_low(x0, p.e1024), a1 = code_low(x1, p.e1024), a2 = code_high(x0, p.e64), a3 = code_high(x1, p.e64);
                         const uint32_t e0 = code_low(y0, p.e1024), e1 = code_low(y1, p.e1024), e2 = code_high(y0, p.e64), e3 = code_high(y1, p.e64);
-                        mma16816_first(part, a0, a1, a2, a3, qf[b + j][2], qf[b + j][3]);   // the small parts first
-                        mma16816(part, e0, e1, e2, e3, qf[b + j][6], qf[b + j][7]);
-                        mma16816(part, a0, a1, a2, a3, qf[b + j][0], qf[b + j][1]);
-                        mma16816(part, e0, e1, e2, e3, qf[b + j][4], qf[b + j][5]);
+                        uint4 lo;
+                        if constexpr (G::kShareQueries) {
+                            lo = s_q[(b + j) * 64 + 32 + lane];
+                        } else {
+                            const int at = G::kShareQueries ? 0 : b + j;
+                            lo = make_uint4(ql[at][0], ql[at][1], ql[at][2], ql[at][3]);
+                        }
+                        mma16816_first(part, a0, a1, a2, a3, lo.x, lo.y);   // the small parts first
+                        mma16816(part, e0, e1, e2, e3, lo.z, lo.w);
+                        mma16816(part, a0, a1, a2, a3, qh[b + j][0], qh[b + j][1]);
+                        mma16816(part, e0, e1, e2, e3, qh[b + j][2], qh[b + j][3]);
                         const float2 f0 = __half22float2(u32_h2(dk[0][b / 2])), f1 = __half22float2(u32_h2(dk[1][b / 2]));
                         const float d0 = j ? f0.y : f0.x, d1 = j ? f1.y : f1.x;
                         sv[s][0] = fmaf(d0, part[0], sv[s][0]), sv[s][1] = fmaf(d0, part[1], sv[s][1]);
@@ -574,26 +591,24 @@ attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap ma
             }
         };
         // tile `it`'s share of the outputs
-        auto outputs = [&](int it, float r0, float r1) {
+        auto outputs_of = [&](int it, float r0, float r1, auto some_masked) {
+            constexpr bool masked = decltype(some_masked)::value;   // some row does not see some cell of the tile
             const int base = (tile_first + it) * kTileCells;
-            const bool masked = base + kTileCells > lim_min;
-            uint8_t * vt = unit_ready(unit_of_v(tile_no + it, u1 - u0));
+            uint8_t * vt = smem + G::ring + (2 + v_stage) * G::kUnitBytes;
             const uint32_t v_addr = smem_u32(vt) + v_off;
+            v_stage = v_stage + 1 == G::kVStages ? 0 : v_stage + 1;
             uint16_t * dv = reinterpret_cast<uint16_t *>(vt + G::kCodeBytes) + cg * kSlabs * 16 * NB + dg;  // this warp's cells and group
-            const int valid = min(kTileCells, c.x.n - base) - cg * kSlabs * 16;    // of its cells, those that were copied
+            const int valid = masked ? min(kTileCells, c.x.n - base) - cg * kSlabs * 16 : kSlabs * 16;   // of its cells, those that were copied
             uint32_t bad = 0;
-            if (masked) {
-                // Behind the request's last cell lies whatever the memory held, and a cell that some row does not see may
-                // hold no number: this warp's scales of such cells become 0.  (The latter are put back below, for the
-                // rows that see them.)  The ring's next copy into this stage comes after them.
+            if constexpr (masked) {
+                // A cell that some row does not see may hold no number: this warp's scales of such cells become 0, and are
+                // put back below for the rows that see them.  (Behind the request's last cell all bytes are 0.)
 #pragma unroll
                 for (int j = 0; j < kSlabs / 2; ++j) {
                     const int cell = lane + 32 * j;
                     const bool none = (dv[cell * NB] & 0x7c00u) == 0x7c00u;
-                    if (cell < valid && none) bad |= 1u << j;
-                    if (cell >= valid || none) dv[cell * NB] = 0;
+                    if (none) bad |= 1u << j, dv[cell * NB] = 0;
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             }
             constexpr int NH = NT > 4 ? 4 : NT;                 // column blocks at a time (registers)
@@ -609,7 +624,7 @@ attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap ma
                 }
 #pragma unroll
                 for (int sp = 0; sp < kSlabs; sp += 2) {
-                    if (sp * 16 >= valid) break;
+                    if (masked && sp * 16 >= valid) break;
                     uint32_t w[4];  // cells 0-7 and 8-15 of the first slab, then of the second
                     ldm4t(w, v_addr + sp * 16 * (HD / 2));
                     // a 256-wide cell's scales are a matrix row: transposed, lane (g, t) has group g's of cells 2 t, 2 t + 1
@@ -658,7 +673,7 @@ attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap ma
                     }
                 }
             }
-            if (masked && __any_sync(kFull, bad != 0)) {
+            if constexpr (masked) if (__any_sync(kFull, bad != 0)) {
                 for (int cell = 0; cell < kSlabs * 16; ++cell) {
                     if ((__shfl_sync(kFull, bad, cell & 31) >> (cell >> 5) & 1u) == 0) continue;
 #pragma unroll
@@ -674,25 +689,31 @@ attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap ma
             }
         };
 
-        // One barrier a tile: behind it lie the tile's scores and the probabilities of the tile before, and between two
-        // of them a warp has three pieces of work that do not wait for one another.
+        auto outputs = [&](int it, float r0, float r1) {
+            if ((tile_first + it + 1) * kTileCells > lim_min) {
+                outputs_of(it, r0, r1, std::true_type{});
+            } else {
+                outputs_of(it, r0, r1, std::false_type{});
+            }
+        };
+
+        // One barrier a tile: behind it lie the tile's scores, the probabilities of the tile before and all copies begun
+        // before the last barrier.  Between two barriers a warp has three pieces of work that do not wait for one another.
         scores(0);
         float r0 = 0.0f, r1 = 0.0f;
         for (int it = 0; it < n_tiles; ++it) {
+            copies_wait<0>();
             named_barrier<1>(kThreadsC);
-            if (wid == 0) {
-                // no longer read: this tile's K and everything before it in the ring (the V of the tile before is behind it)
-                if (tile_no + uint32_t(it) > 0) feed();
-            }
+            load.next(p, ring);  // into the stages of this tile's K and of the V before the last
             float s0, s1;
             weights(it, s0, s1);
             if (it > 0) outputs(it - 1, r0, r1);
             if (it + 1 < n_tiles) scores(it + 1);
             r0 = s0, r1 = s1;
         }
+        copies_wait<0>();
         named_barrier<1>(kThreadsC);
         outputs(n_tiles - 1, r0, r1);
-        tile_no += uint32_t(n_tiles);
 
         // ---- the item's end: sums across the warps, cell groups joined, rows written or left to be folded
 #pragma unroll
@@ -755,23 +776,20 @@ attend_paged_kernel(const paged_params p, const __grid_constant__ CUtensorMap ma
         u += uint32_t(n_tiles);
         if (u < u1) c.next_item(p);
     }
-    // after a wait that ran out: every copy has landed before the CTA's shared memory can be handed on
-    if (tid == 0) {
-        const uint32_t done = s_feed->step, k = done == 0 ? 0 : done > s_feed->tiles_all ? 2 * s_feed->tiles_all : 2 * done - 1;  // units issued
-        for (uint32_t j = 1; j <= uint32_t(G::kRing) && j <= k; ++j) mbar_wait_landed(&full[(k - j) % G::kRing], ((k - j) / G::kRing) & 1u);
-    }
 }
 
 // ---- the fold -----------------------------------------------------------------------------------------------------------
 // Block (i, col): if piece i + 1 is the second of an item's, the item's pieces are folded for one column:
 // weights 2^(m - max), accumulators and sums joined in the order of the pieces, eight warps taking every eighth piece.
 constexpr int kFoldWarps = 8;
+constexpr int kMaxPieces = 2 * kSmCount;
 template <int HD, int NT>
 __global__ void __launch_bounds__(kFoldWarps * 32) attend_paged_fold_kernel(const paged_params p) {
     constexpr int COLS = 8 * NT, V = HD / 128 > 0 ? HD / 128 : 1;   // float4 vectors of a lane
     constexpr int LANES = HD / 4 < 32 ? HD / 4 : 32;
     __shared__ float4 s_acc[kFoldWarps][HD / 4];
     __shared__ float s_max[kFoldWarps], s_sum[kFoldWarps];
+    __shared__ float s_weight[kMaxPieces], s_part[kMaxPieces];
     pdl_launch_dependents();
     pdl_wait();
     const int col = blockIdx.y;
@@ -781,51 +799,57 @@ __global__ void __launch_bounds__(kFoldWarps * 32) attend_paged_fold_kernel(cons
     const int row = (f.blk * COLS + col) / p.group;
     if (row >= x.m) return;
 
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    float4 acc[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    float m = -INFINITY, l = 0.0f;
-    // the pieces after the first hold the item from their start: slot 0; in the first it is the last: slot 1
-#pragma unroll 4
-    for (int j = f.from + wid; j <= f.to; j += kFoldWarps) {
-        const int64_t slot = int64_t(j) * 2 + (j == f.from ? 1 : 0);
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.ws_ml + (slot * COLS + col) * 2));
-        float4 a[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            a[v] = lane < LANES ? __ldcg(reinterpret_cast<const float4 *>(p.ws_acc + (slot * COLS + col) * HD) + lane + 32 * v)
-                                : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.0f : top;
-        const float wo = ex2(m - base), wn = ex2(ml.x - base);
-        m = top;
-        l = fmaf(l, wo, ml.y * wn);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            acc[v].x = fmaf(acc[v].x, wo, a[v].x * wn), acc[v].y = fmaf(acc[v].y, wo, a[v].y * wn);
-            acc[v].z = fmaf(acc[v].z, wo, a[v].z * wn), acc[v].w = fmaf(acc[v].w, wo, a[v].w * wn);
-        }
-    }
-    if (lane < LANES) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) s_acc[wid][lane + 32 * v] = acc[v];
-    }
-    if (lane == 0) s_max[wid] = m, s_sum[wid] = l;
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= HD) return;
+    // weights of the pieces, then one pass over their accumulators.  The pieces after the first hold the item from their
+    // start: slot 0; in the first it is the last: slot 1.
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, n = f.to - f.from + 1;
+    auto slot_of = [&](int j) { return (int64_t(f.from + j) * 2 + (j == 0 ? 1 : 0)) * COLS + col; };
     float top = -INFINITY;
+    for (int j = threadIdx.x; j < n; j += kFoldWarps * 32) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.ws_ml + slot_of(j) * 2));
+        s_weight[j] = ml.x, s_part[j] = ml.y;
+        top = fmaxf(top, ml.x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+    if (lane == 0) s_max[wid] = top;
+    __syncthreads();
 #pragma unroll
     for (int w = 0; w < kFoldWarps; ++w) top = fmaxf(top, s_max[w]);
     const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    for (int j = threadIdx.x; j < n; j += kFoldWarps * 32) {
+        const float w = ex2(s_weight[j] - base);
+        s_weight[j] = w;
+        sum = fmaf(s_part[j], w, sum);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    if (lane == 0) s_sum[wid] = sum;
+    __syncthreads();
+    float4 acc[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (lane < LANES) {
+#pragma unroll 8
+        for (int j = wid; j < n; j += kFoldWarps) {
+            const float w = s_weight[j];
+            const float4 * src = reinterpret_cast<const float4 *>(p.ws_acc + slot_of(j) * HD) + lane;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float4 a = __ldcg(src + 32 * v);
+                acc[v].x = fmaf(a.x, w, acc[v].x), acc[v].y = fmaf(a.y, w, acc[v].y);
+                acc[v].z = fmaf(a.z, w, acc[v].z), acc[v].w = fmaf(a.w, w, acc[v].w);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) s_acc[wid][lane + 32 * v] = acc[v];
+    }
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= HD) return;
     float a = 0.0f, s = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kFoldWarps; ++w) {
-        const float k = ex2(s_max[w] - base);
-        a = fmaf(reinterpret_cast<const float *>(s_acc[w])[d], k, a);
-        s = fmaf(s_sum[w], k, s);
-    }
+    for (int w = 0; w < kFoldWarps; ++w) a += reinterpret_cast<const float *>(s_acc[w])[d], s += s_sum[w];
     float y = s == 0.0f ? 0.0f : __fdiv_rn(a, s);
     const int64_t at = (int64_t(x.row0 + row) * p.n_q + f.h * p.group + (f.blk * COLS + col) % p.group) * HD + d;
     if (p.gate != nullptr) y = __fdiv_rn(y, 1.0f + expf(-__ldg(p.gate + at)));
@@ -833,34 +857,6 @@ __global__ void __launch_bounds__(kFoldWarps * 32) attend_paged_fold_kernel(cons
 }
 
 // ---- launch -------------------------------------------------------------------------------------------------------------
-using encode_fn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                               const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-encode_fn encode_tensor_map() {
-    static const encode_fn fn = [] {
-        void * f = nullptr;
-        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
-            (void) cudaGetLastError();
-            return encode_fn(nullptr);
-        }
-        return reinterpret_cast<encode_fn>(f);
-    }();
-    return fn;
-}
-// a plane's codes [kv head][slot][hd / 2 bytes], 16 bits an element; the box one page (at most a tile) of one head, its
-// cells' 16-byte chunks swizzled over the whole cell
-bool make_map(CUtensorMap * map, const void * codes, int64_t slots, int n_kv, int hd, int box) {
-    const encode_fn enc = encode_tensor_map();
-    if (enc == nullptr) return false;
-    const cuuint64_t dims[3] = {cuuint64_t(hd / 4), cuuint64_t(slots), cuuint64_t(n_kv)};
-    const cuuint64_t strides[2] = {cuuint64_t(hd / 2), cuuint64_t(slots) * cuuint64_t(hd / 2)};
-    const cuuint32_t boxes[3] = {cuuint32_t(hd / 4), cuuint32_t(box), 1u}, elem[3] = {1u, 1u, 1u};
-    const CUtensorMapSwizzle swz = hd == 256 ? CU_TENSOR_MAP_SWIZZLE_128B : hd == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
-    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(codes), dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               swz, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int HD, int NT>
 bool configure() {
     static std::atomic<bool> done[64];
@@ -899,17 +895,13 @@ bool paged_shape_ok(const fnb_attend_paged_args * a) {
     if (a->n_q_heads < 1 || a->n_kv_heads < 1 || a->n_q_heads > 1024 || a->n_q_heads % a->n_kv_heads != 0) return false;
     if (a->page_size < 16 || a->page_size > (1 << 20) || (a->page_size & (a->page_size - 1)) != 0) return false;
     if (a->cache_slots < a->page_size || a->cache_slots > INT32_MAX || a->cache_slots % a->page_size != 0) return false;
+    if (a->cache_slots * a->n_kv_heads > int64_t(UINT32_MAX)) return false;
     return true;
 }
 
 template <int HD, int NT>
 int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStream_t s) {
-    const int box = a->page_size < kTileCells ? a->page_size : kTileCells;
-    CUtensorMap map_k, map_v;
-    if (!make_map(&map_k, a->k_cache, a->cache_slots, a->n_kv_heads, HD, box) || !make_map(&map_v, a->v_cache, a->cache_slots, a->n_kv_heads, HD, box) ||
-        !configure<HD, NT>()) {
-        return FNB_LAUNCH_FAILED;
-    }
+    if (!configure<HD, NT>()) return FNB_LAUNCH_FAILED;
     const int grid = ctas_of(NT);
     const size_t cols = 8 * NT;
     const bool fold = !one_tile(a);
@@ -919,7 +911,7 @@ int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStre
         p.ws_acc = reinterpret_cast<float *>(ws + size_t(grid) * 32);
         p.ws_ml = p.ws_acc + size_t(grid) * 2 * cols * HD;
     }
-    launch_pdl(attend_paged_kernel<HD, NT>, grid, kThreadsC, geo<HD, NT>::total, s, p, map_k, map_v);
+    launch_pdl(attend_paged_kernel<HD, NT>, grid, kThreadsC, geo<HD, NT>::total, s, p);
     if (cudaPeekAtLastError() != cudaSuccess) return FNB_LAUNCH_FAILED;
     if (fold) {
         cudaLaunchConfig_t cfg = {};
@@ -947,7 +939,6 @@ bool prepare_hd() { return configure<HD, 1>() && configure<HD, 2>() && configure
 }  // namespace
 
 bool attend_paged_prepare_device() {
-    (void) encode_tensor_map();
     return prepare_hd<256>() && prepare_hd<128>() && prepare_hd<64>();
 }
 
@@ -968,6 +959,7 @@ extern "C" int32_t fnb_attend_paged_kv4(const fnb_attend_paged_args * a, void * 
     if (!(a->scale > 0.0f) || !(a->scale < INFINITY)) return FNB_REJECTED;
     if (!one_tile(a) && (!ok_ptr(a->workspace, 16) || a->workspace_bytes < paged_workspace(a))) return FNB_REJECTED;
     paged_params p = {};
+    p.k_cache = static_cast<const uint8_t *>(a->k_cache), p.v_cache = static_cast<const uint8_t *>(a->v_cache);
     p.q = a->q, p.gate = a->gate, p.k_scale = a->k_scale, p.v_scale = a->v_scale;
     p.table = a->table, p.n_cells = a->n_cells, p.row_start = a->row_start, p.out = a->out, p.err = a->err;
     p.cache_slots = a->cache_slots, p.rows = a->rows, p.n_req = a->n_req, p.max_pages = a->max_pages;
