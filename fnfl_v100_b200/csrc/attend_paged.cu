@@ -62,16 +62,18 @@ struct geo {
     static constexpr int kCodeBytes = kTileCells * HD / 2, kScaleBytes = kTileCells * kGroups * 2;
     static constexpr int kUnitBytes = kCodeBytes + kScaleBytes;
     static constexpr int kCtas = NT <= 2 ? 2 : 1;               // resident on an SM (registers)
-    static constexpr int kVStages = 3, kStages = 2 + kVStages;   // K's, then V's
+    // V is put out a tile behind K, so a third stage lets its copies begin a tile earlier; two where the memory is short
+    static constexpr int kVStages = NT == 1 || NT == 4 ? 3 : 2, kStages = 2 + kVStages;   // K's stages, then V's
+    // scores: a warp's slabs of 16 cells and column blocks.  With many columns two slabs share a fragment's load.
+    static constexpr int kSlabsW = NT >= 4 ? 2 : 1, kBlocksW = NT / kSlabsW, kSlabGroups = 8 / kSlabsW;
     static constexpr uint32_t kSwz = HD == 256 ? 7u : HD == 128 ? 3u : 1u;
     // shared memory
     static constexpr int ring = 0;
     static constexpr int prob = ring + kStages * kUnitBytes;    // uint4 [2][8 slabs][NT][32]
-    static constexpr bool kShareQueries = NT == 1;              // one column block: every warp has the same fragments
-    static constexpr int qfrag = prob + 2 * 8 * NT * 512;       // uint4 [kGroups][hi, lo][32]
-    static constexpr int wmax = qfrag + (kShareQueries ? kGroups * 1024 : 0);  // float [2][8 warps][8]
-    static constexpr int lsum = wmax + 512;                     // float [8 warps][8]
-    static constexpr int corr = lsum + 256;                     // float [2][kCols]
+    static constexpr int qfrag = prob + 2 * 8 * NT * 512;       // uint4 [NT][kGroups][hi, lo][32]
+    static constexpr int wmax = qfrag + NT * kGroups * 1024;    // float [2][kSlabGroups][kCols]; and the queries' [kGroups][kCols]
+    static constexpr int lsum = wmax + 2 * 8 * kCols * 4;       // float [kSlabGroups][kCols]
+    static constexpr int corr = lsum + 8 * kCols * 4;           // float [2][kCols]
     static constexpr int mfin = corr + 2 * kCols * 4;           // float [kCols]
     static constexpr int red = mfin + kCols * 4;                // float4: the other cell groups' accumulators
     static constexpr int scan = red + (kCellGroups - 1) * kGroups * 32 * kCols * 4;  // int64 [8]: sums; the piece's start
@@ -87,6 +89,7 @@ struct paged_params {
     float * out;
     float *ws_acc, *ws_ml;
     int32_t * ws_head;  // [grid][8]: what the fold has to do at the start of each piece (fold_head)
+    int32_t * ws_mark;  // [grid]: whether that is anything
     uint32_t * err;
     int64_t cache_slots;
     int cells_max;      // what a table row can list
@@ -228,20 +231,21 @@ struct fold_head {
 };
 
 // ---- the copies -------------------------------------------------------------------------------------------------------
-// Step s of a piece brings tile s's K and tile s - 1's V.  A warp copies sixteen rows, which lie in one page: one page id
-// a warp and tile, fetched a step ahead, and addresses that differ by constants.  A lane copies one 16-byte chunk (a
+// Step s of a piece brings tile s's K and tile s - kLag's V.  A warp copies sixteen rows, which lie in one page: one page
+// id a warp and tile, fetched a step ahead, and addresses that differ by constants.  A lane copies one 16-byte chunk (a
 // group's codes) of kPass rows, and one row's scales, K's (lower half-warp) or V's.  Chunk c of a row lies at c ^ (bits
 // of the row), which keeps ldmatrix free of bank conflicts.  The walk runs two tiles ahead of the scores.
 template <int HD, int NT>
 struct loader {
     using G = geo<HD, NT>;
     static constexpr int kCh = G::kGroups, kRows = 32 / kCh, kPass = 16 / kRows, kRow = HD / 2, kScale = kCh * 2;
+    static constexpr int kLag = 4 - G::kVStages;
     cursor<G::kCols> c;
     uint32_t step, tiles;  // of the piece
     uint32_t v_stage;
     int32_t id;            // page of the warp's rows in tile `step`
-    uint32_t cell;         // first of its rows in tile `step` - 1, counted through all heads of a plane
-    int v_left;            // that tile's cells from the warp's first row on
+    uint32_t cell[kLag];   // first of its rows in the kLag tiles before `step` (the last first), counted through all heads of a plane
+    int left[kLag];        // those tiles' cells from the warp's first row on
     uint32_t lane_to;      // this lane's chunk of the warp's first pass within a stage
 
     __device__ __forceinline__ static int warp_row() { return int(threadIdx.x >> 5) * 16; }
@@ -250,50 +254,54 @@ struct loader {
         id = at < c.x.n ? __ldg(p.table + int64_t(c.r) * p.max_pages + (at >> p.page_shift)) : 0;
     }
     __device__ __forceinline__ void start(const paged_params & p, const cursor<G::kCols> & from, uint32_t n) {
-        c = from, step = 0, tiles = n, v_stage = G::kVStages - 1, v_left = 0, cell = 0;
+        c = from, step = 0, tiles = n, v_stage = 0;
+#pragma unroll
+        for (int i = 0; i < kLag; ++i) cell[i] = 0, left[i] = 0;
         fetch(p);
         const uint32_t lane = threadIdx.x & 31, row = uint32_t(warp_row()) + lane / kCh;
         lane_to = row * kRow + (((lane % kCh) ^ ((row * kRow >> 7) & G::kSwz)) << 4);
     }
-    // `left` (at most sixteen count) of the rows at cell `first` into the stage at `st`
-    __device__ __forceinline__ void rows(const uint8_t * plane, uint32_t first, int left, uint32_t st) const {
+    // `some` (at most sixteen count) of the rows at cell `first` into the stage at `st`
+    __device__ __forceinline__ void rows(const uint8_t * plane, uint32_t first, int some, uint32_t st) const {
         const uint32_t lane = threadIdx.x & 31;
         const uint8_t * src = plane + uint64_t(first) * kRow + lane * 16;
         const uint32_t to = st + lane_to;
         // a 256-wide cell: four rows a pass, so every second pass has the other half of the eight row patterns
-        if (left >= 16) {
+        if (some >= 16) {
 #pragma unroll
             for (int i = 0; i < kPass; ++i) copy_async<16>((to + i * kRows * kRow) ^ (kRows == 4 && (i & 1) ? 64u : 0u), src + i * kRows * kRow, true);
         } else {
 #pragma unroll
             for (int i = 0; i < kPass; ++i) {
-                copy_async<16>((to + i * kRows * kRow) ^ (kRows == 4 && (i & 1) ? 64u : 0u), src + i * kRows * kRow, int(lane / kCh) + i * kRows < left);
+                copy_async<16>((to + i * kRows * kRow) ^ (kRows == 4 && (i & 1) ? 64u : 0u), src + i * kRows * kRow, int(lane / kCh) + i * kRows < some);
             }
         }
     }
     __device__ __forceinline__ void next(const paged_params & p, uint32_t ring) {
-        if (step > tiles) return;
+        if (step >= tiles + kLag) return;
         const uint32_t lane = threadIdx.x & 31;
-        const bool k_too = step < tiles, v_too = step > 0;
+        const bool k_too = step < tiles, v_too = step >= uint32_t(kLag);
         const uint32_t k_st = ring + (step & 1) * G::kUnitBytes, v_st = ring + (2 + v_stage) * G::kUnitBytes;
-        const uint32_t v_cell = cell;
-        const int old_left = v_left;
-        if (v_too) rows(p.v_cache, v_cell, old_left, v_st);
+        const uint32_t v_cell = cell[kLag - 1];
+        const int v_left = left[kLag - 1];
+        if (v_too) rows(p.v_cache, v_cell, v_left, v_st);
+#pragma unroll
+        for (int i = kLag - 1; i > 0; --i) cell[i] = cell[i - 1], left[i] = left[i - 1];
         if (k_too) {
             const int base = c.tile * kTileCells + warp_row();
-            v_left = c.x.n - base;
+            left[0] = c.x.n - base;
             if (uint32_t(id) >= uint32_t(p.n_pages)) {
                 if (lane == 0 && p.err != nullptr) atomicOr(p.err, FNB_ERR_PAGES);
                 id = 0;
             }
-            cell = uint32_t(c.h) * uint32_t(p.cache_slots) + (uint32_t(id) << p.page_shift) + (uint32_t(base) & ((1u << p.page_shift) - 1));
-            rows(p.k_cache, cell, v_left, k_st);
+            cell[0] = uint32_t(c.h) * uint32_t(p.cache_slots) + (uint32_t(id) << p.page_shift) + (uint32_t(base) & ((1u << p.page_shift) - 1));
+            rows(p.k_cache, cell[0], left[0], k_st);
         }
         const bool lower = lane < 16;
         if (lower ? k_too : v_too) {
-            const uint32_t at = (lower ? cell : v_cell) + (lane & 15);
+            const uint32_t at = (lower ? cell[0] : v_cell) + (lane & 15);
             copy_async<kScale>((lower ? k_st : v_st) + G::kCodeBytes + uint32_t(warp_row() + (lane & 15)) * kScale,
-                               (lower ? p.k_scale : p.v_scale) + uint64_t(at) * kCh, int(lane & 15) < (lower ? v_left : old_left));
+                               (lower ? p.k_scale : p.v_scale) + uint64_t(at) * kCh, int(lane & 15) < (lower ? left[0] : v_left));
         }
         copies_commit();
         if (step + 1 < tiles) {
@@ -301,7 +309,7 @@ struct loader {
             fetch(p);
         }
         ++step;
-        v_stage = v_stage + 1 == G::kVStages ? 0 : v_stage + 1;
+        if (v_too) v_stage = v_stage + 1 == G::kVStages ? 0 : v_stage + 1;
     }
 };
 
@@ -362,7 +370,10 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     }
     __syncthreads();
     if (u0 >= u1) {
-        if (tid == 0 && p.ws_head != nullptr) reinterpret_cast<fold_head *>(p.ws_head + int64_t(blockIdx.x) * 8)->fold = 0;
+        if (tid == 0 && p.ws_head != nullptr) {
+            reinterpret_cast<fold_head *>(p.ws_head + int64_t(blockIdx.x) * 8)->fold = 0;
+            p.ws_mark[blockIdx.x] = 0;
+        }
         return;
     }
     cursor<G::kCols> c;
@@ -378,10 +389,12 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             f.fold = int(blockIdx.x) == f.from + 1;                // a cut piece is never empty, so neither is the next
         }
         *reinterpret_cast<fold_head *>(p.ws_head + int64_t(blockIdx.x) * 8) = f;
+        p.ws_mark[blockIdx.x] = f.fold;
     }
 
     const int g = lane >> 2, t = lane & 3;
-    const int nt = wid % NT, slab0 = wid / NT * NT;                  // scores: column block and first of NT slabs
+    constexpr int SL = G::kSlabsW, NW = G::kBlocksW;
+    const int sg = wid / SL, x_first = wid % SL;                     // scores: slab group; column blocks x_first, + SL, ..
     const int dg = wid % NB, cg = wid / NB;                          // outputs: dim group, cell group
     constexpr int kSlabs = 8 / G::kCellGroups;                       // slabs of a cell group
     float * s_wmax = reinterpret_cast<float *>(smem + G::wmax);
@@ -394,7 +407,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     // (the same for every sixteenth row, so all addresses of a lane differ by constants)
     const int lrow = (lane & 7) + ((lane >> 3) & 1) * 8, lhalf = lane >> 4;
     const uint32_t swz = (uint32_t(lrow) * (HD / 2) >> 7) & G::kSwz;
-    const uint32_t k_off = uint32_t(slab0 * 16 + lrow) * (HD / 2) + ((uint32_t(lhalf) ^ swz) << 4);                 // groups 0, 1
+    const uint32_t k_off = uint32_t(sg * SL * 16 + lrow) * (HD / 2) + ((uint32_t(lhalf) ^ swz) << 4);               // groups 0, 1
     const uint32_t v_off = uint32_t(cg * kSlabs * 16 + lhalf * 16 + lrow) * (HD / 2) + ((uint32_t(dg) ^ swz) << 4);  // slabs 0, 1
 
     uint32_t k_stage = 0, v_stage = 0;  // of the next tile scored, of the next tile put out
@@ -406,91 +419,81 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         const int col0 = c.blk * G::kCols;
         auto row_of_col = [&](int col) { return (col0 + col) / p.group; };
 
-        // Queries of column 8 nt + g, split, in the order of the fragments: dims 8 t + {0, 4}, {1, 5}, {2, 6}, {3, 7} of a
-        // group, which are nibbles 0 .. 3 of the two halves of a cell's word.
-        uint32_t qh[NB][4];                                  // hi parts
-        uint32_t ql[G::kShareQueries ? 1 : NB][4];           // lo parts
-        float sc0, sc1;
-        int lim0, lim1;
-        {
-            const int col = nt * 8 + g, i = row_of_col(col);
+        const int n_blocks = min(NT, (c.x.m * p.group - col0 + 7) / 8);   // column blocks with a live column
+        // Queries, split, in the order of the fragments: lane (g, t) has dims 8 t + {0, 4}, {1, 5}, {2, 6}, {3, 7} of a group
+        // of column 8 x + g, which are nibbles 0 .. 3 of the two halves of a cell's word.  A (column block, group) at a time
+        // a warp; the rows' maxima and then the fragments cross the warps.
+        auto load8 = [&](int b, int x, float4 (&v)[2]) {
+            const int col = x * 8 + g, i = row_of_col(col);
+            const float * src = p.q + (int64_t(c.x.row0 + i) * p.n_q + c.h * p.group + (col0 + col - i * p.group)) * HD + 32 * b + 8 * t;
             const bool on = i < c.x.m;
-            const float * src = p.q + (int64_t(c.x.row0 + (on ? i : 0)) * p.n_q + c.h * p.group + (col0 + col) % p.group) * HD + 8 * t;
-            const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-            auto load8 = [&](int b, float4 (&v)[2]) {
-                v[0] = on ? __ldg(reinterpret_cast<const float4 *>(src + 32 * b)) : zero;
-                v[1] = on ? __ldg(reinterpret_cast<const float4 *>(src + 32 * b + 4)) : zero;
-            };
-            auto top8 = [&](const float4 (&v)[2]) {
-                return fmaxf(fmaxf(fmaxf(fabsf(v[0].x), fabsf(v[0].y)), fmaxf(fabsf(v[0].z), fabsf(v[0].w))),
-                             fmaxf(fmaxf(fabsf(v[1].x), fabsf(v[1].y)), fmaxf(fabsf(v[1].z), fabsf(v[1].w))));
-            };
-            auto split8 = [&](const float4 (&v)[2], float up, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-                split2(__fmul_rn(v[0].x, up), __fmul_rn(v[1].x, up), hi[0], lo[0]);
-                split2(__fmul_rn(v[0].y, up), __fmul_rn(v[1].y, up), hi[1], lo[1]);
-                split2(__fmul_rn(v[0].z, up), __fmul_rn(v[1].z, up), hi[2], lo[2]);
-                split2(__fmul_rn(v[0].w, up), __fmul_rn(v[1].w, up), hi[3], lo[3]);
-            };
-            // the power of two that takes the row's largest into [2^13, 2^14), and its inverse
-            auto powers = [&](float top, float & up, float & down) {
-                int e = int(__float_as_uint(top) >> 23);
-                e = e < 14 ? 14 : e > 254 ? 254 : e;
-                up = __uint_as_float(uint32_t(267 - e) << 23), down = __uint_as_float(uint32_t(e - 13) << 23);
-            };
+            v[0] = on ? __ldg(reinterpret_cast<const float4 *>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[1] = on ? __ldg(reinterpret_cast<const float4 *>(src + 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        auto powers = [&](float top, float & up, float & down) {  // the power of two that takes top into [2^13, 2^14), its inverse
+            int e = int(__float_as_uint(top) >> 23);
+            e = e < 14 ? 14 : e > 254 ? 254 : e;
+            up = __uint_as_float(uint32_t(267 - e) << 23), down = __uint_as_float(uint32_t(e - 13) << 23);
+        };
+        auto top_of = [&](int col) {
+            float top = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) top = fmaxf(top, s_wmax[b * G::kCols + col]);
+            return top;
+        };
+        constexpr int kPairs = NB * NT;
+        float4 first[2];
+        if (wid < kPairs) load8(wid % NB, wid / NB, first);
+        if (load.step == 0) load.next(p, ring);              // the piece's first copies, while the queries arrive
+#pragma unroll
+        for (int k = 0; k * kWarpsC < kPairs; ++k) {
+            const int pair = wid + k * kWarpsC, b = pair % NB, x = pair / NB;
+            if (pair >= kPairs) break;
+            float4 v[2] = {first[0], first[1]};
+            if (k > 0) load8(b, x, v);
+            float top = fmaxf(fmaxf(fmaxf(fabsf(v[0].x), fabsf(v[0].y)), fmaxf(fabsf(v[0].z), fabsf(v[0].w))),
+                              fmaxf(fmaxf(fabsf(v[1].x), fabsf(v[1].y)), fmaxf(fabsf(v[1].z), fabsf(v[1].w))));
+            top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+            if (t == 0) s_wmax[b * G::kCols + x * 8 + g] = top;
+        }
+        if (load.step == 1) load.next(p, ring);
+        named_barrier<1>(kThreadsC);
+#pragma unroll
+        for (int k = 0; k * kWarpsC < kPairs; ++k) {
+            const int pair = wid + k * kWarpsC, b = pair % NB, x = pair / NB;
+            if (pair >= kPairs) break;
+            float4 v[2] = {first[0], first[1]};
+            if (k > 0) load8(b, x, v);                       // again, from L1
             float up, down;
-            if constexpr (G::kShareQueries) {
-                // a group a warp; the maxima and then the fragments cross the warps
-                float4 v[2] = {zero, zero};
-                if (wid < NB) load8(wid, v);
-                if (load.step == 0) load.next(p, ring);      // the piece's first copies, while the queries arrive
-                float top = top8(v);
-                top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-                if (t == 0) s_wmax[wid * 8 + g] = top;
-                if (load.step == 1) load.next(p, ring);
-                named_barrier<1>(kThreadsC);
-                top = 0.0f;
+            powers(top_of(x * 8 + g), up, down);
+            uint4 hi, lo;
+            split2(__fmul_rn(v[0].x, up), __fmul_rn(v[1].x, up), hi.x, lo.x);
+            split2(__fmul_rn(v[0].y, up), __fmul_rn(v[1].y, up), hi.y, lo.y);
+            split2(__fmul_rn(v[0].z, up), __fmul_rn(v[1].z, up), hi.z, lo.z);
+            split2(__fmul_rn(v[0].w, up), __fmul_rn(v[1].w, up), hi.w, lo.w);
+            s_q[(x * NB + b) * 64 + lane] = hi, s_q[(x * NB + b) * 64 + 32 + lane] = lo;
+        }
+        // this warp's columns: the factor of their scores, the cells they see; running maxima and sums
+        float sc[NW][2], mx[NW][2], ls[NW][2];
+        int lim[NW][2];
 #pragma unroll
-                for (int b = 0; b < NB; ++b) top = fmaxf(top, s_wmax[b * 8 + g]);
-                powers(top, up, down);
-                if (wid < NB) {
-                    uint32_t hi[4], lo[4];
-                    split8(v, up, hi, lo);
-                    s_q[wid * 64 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    s_q[wid * 64 + 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                }
-                copies_wait<1>();                            // K of the piece's first tile
-                named_barrier<1>(kThreadsC);
+        for (int i = 0; i < NW; ++i) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const uint4 v4 = s_q[b * 64 + lane];
-                    qh[b][0] = v4.x, qh[b][1] = v4.y, qh[b][2] = v4.z, qh[b][3] = v4.w;
-                }
-            } else {
-                while (load.step < 2 && load.step <= u1 - u0) load.next(p, ring);
-                float4 v[NB][2];
-                float top = 0.0f;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) load8(b, v[b]);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) top = fmaxf(top, top8(v[b]));
-                top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-                powers(top, up, down);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) split8(v[b], up, qh[b], ql[G::kShareQueries ? 0 : b]);
-                copies_wait<1>();
-                named_barrier<1>(kThreadsC);
+            for (int z = 0; z < 2; ++z) {
+                const int col = (x_first + i * SL) * 8 + 2 * t + z, r = row_of_col(col);
+                float up, down;
+                powers(top_of(col), up, down);
+                sc[i][z] = fmaxf(p.scale_log2 * down, 0x1p-126f);
+                lim[i][z] = r < c.x.m ? c.x.n - c.x.m + r + 1 : 0;
+                mx[i][z] = -INFINITY, ls[i][z] = 0.0f;
             }
-            const float sc = fmaxf(p.scale_log2 * down, 0x1p-126f);
-            sc0 = __shfl_sync(kFull, sc, 8 * t), sc1 = __shfl_sync(kFull, sc, 8 * t + 4);
-            const int i0 = row_of_col(nt * 8 + 2 * t), i1 = row_of_col(nt * 8 + 2 * t + 1);
-            lim0 = i0 < c.x.m ? c.x.n - c.x.m + i0 + 1 : 0, lim1 = i1 < c.x.m ? c.x.n - c.x.m + i1 + 1 : 0;
         }
         const int lim_min = c.x.n - c.x.m + row_of_col(0) + 1;   // cells every live row of the block sees
+        copies_wait<1>();                                        // K of the piece's first tile
+        named_barrier<1>(kThreadsC);
 
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-        float sv[NT][4];
+        float sv[SL][NW][4];
         float acc[NT][2][4];
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
@@ -507,87 +510,120 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             const uint8_t * kt = smem + G::ring + k_stage * G::kUnitBytes;
             const uint32_t k_addr = ring + k_stage * G::kUnitBytes + k_off;
             k_stage ^= 1;
+            uint32_t dk[SL][2][NB / 2];
 #pragma unroll
-            for (int s = 0; s < NT; ++s) {
-                const int row = (slab0 + s) * 16;
-                const uint8_t * at0 = kt + G::kCodeBytes + (row + g) * (NB * 2), * at1 = at0 + 8 * NB * 2;
-                sv[s][0] = sv[s][1] = sv[s][2] = sv[s][3] = 0.0f;
-                uint32_t dk[2][NB / 2];
-                if constexpr (NB == 8) {
-                    *reinterpret_cast<uint4 *>(dk[0]) = *reinterpret_cast<const uint4 *>(at0);
-                    *reinterpret_cast<uint4 *>(dk[1]) = *reinterpret_cast<const uint4 *>(at1);
-                } else if constexpr (NB == 4) {
-                    *reinterpret_cast<uint2 *>(dk[0]) = *reinterpret_cast<const uint2 *>(at0);
-                    *reinterpret_cast<uint2 *>(dk[1]) = *reinterpret_cast<const uint2 *>(at1);
-                } else {
-                    *reinterpret_cast<uint32_t *>(dk[0]) = *reinterpret_cast<const uint32_t *>(at0);
-                    *reinterpret_cast<uint32_t *>(dk[1]) = *reinterpret_cast<const uint32_t *>(at1);
+            for (int s = 0; s < SL; ++s) {
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    const uint8_t * at = kt + G::kCodeBytes + ((sg * SL + s) * 16 + g + 8 * z) * (NB * 2);
+                    if constexpr (NB == 8) {
+                        *reinterpret_cast<uint4 *>(dk[s][z]) = *reinterpret_cast<const uint4 *>(at);
+                    } else if constexpr (NB == 4) {
+                        *reinterpret_cast<uint2 *>(dk[s][z]) = *reinterpret_cast<const uint2 *>(at);
+                    } else {
+                        *reinterpret_cast<uint32_t *>(dk[s][z]) = *reinterpret_cast<const uint32_t *>(at);
+                    }
                 }
 #pragma unroll
-                for (int b = 0; b < NB; b += 2) {
+                for (int i = 0; i < NW; ++i) sv[s][i][0] = sv[s][i][1] = sv[s][i][2] = sv[s][i][3] = 0.0f;
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b += 2) {
+                uint32_t ka[SL][2][8];  // two groups' operands: nibbles 0 and 1, then 2 and 3
+#pragma unroll
+                for (int s = 0; s < SL; ++s) {
                     uint32_t w[4];
                     ldm4(w, (k_addr + s * 16 * (HD / 2)) ^ uint32_t(b << 4));
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float part[4];
                         const uint32_t x0 = w[2 * j], x1 = w[2 * j + 1], y0 = x0 >> 8, y1 = x1 >> 8;
-                        const uint32_t a0 = code_low(x0, p.e1024), a1 = code_low(x1, p.e1024), a2 = code_high(x0, p.e64), a3 = code_high(x1, p.e64);
-                        const uint32_t e0 = code_low(y0, p.e1024), e1 = code_low(y1, p.e1024), e2 = code_high(y0, p.e64), e3 = code_high(y1, p.e64);
-                        uint4 lo;
-                        if constexpr (G::kShareQueries) {
-                            lo = s_q[(b + j) * 64 + 32 + lane];
-                        } else {
-                            const int at = G::kShareQueries ? 0 : b + j;
-                            lo = make_uint4(ql[at][0], ql[at][1], ql[at][2], ql[at][3]);
-                        }
-                        mma16816_first(part, a0, a1, a2, a3, lo.x, lo.y);   // the small parts first
-                        mma16816(part, e0, e1, e2, e3, lo.z, lo.w);
-                        mma16816(part, a0, a1, a2, a3, qh[b + j][0], qh[b + j][1]);
-                        mma16816(part, e0, e1, e2, e3, qh[b + j][2], qh[b + j][3]);
-                        const float2 f0 = __half22float2(u32_h2(dk[0][b / 2])), f1 = __half22float2(u32_h2(dk[1][b / 2]));
-                        const float d0 = j ? f0.y : f0.x, d1 = j ? f1.y : f1.x;
-                        sv[s][0] = fmaf(d0, part[0], sv[s][0]), sv[s][1] = fmaf(d0, part[1], sv[s][1]);
-                        sv[s][2] = fmaf(d1, part[2], sv[s][2]), sv[s][3] = fmaf(d1, part[3], sv[s][3]);
+                        ka[s][j][0] = code_low(x0, p.e1024), ka[s][j][1] = code_low(x1, p.e1024);
+                        ka[s][j][2] = code_high(x0, p.e64), ka[s][j][3] = code_high(x1, p.e64);
+                        ka[s][j][4] = code_low(y0, p.e1024), ka[s][j][5] = code_low(y1, p.e1024);
+                        ka[s][j][6] = code_high(y0, p.e64), ka[s][j][7] = code_high(y1, p.e64);
                     }
                 }
-                if (base + kTileCells > lim_min) {
-                    const int cell = base + row + g;
-                    if (cell >= lim0) sv[s][0] = -INFINITY;
-                    if (cell >= lim1) sv[s][1] = -INFINITY;
-                    if (cell + 8 >= lim0) sv[s][2] = -INFINITY;
-                    if (cell + 8 >= lim1) sv[s][3] = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NW; ++i) {
+                    const int x = x_first + i * SL;
+                    if (NT > 1 && x >= n_blocks) break;
+                    uint4 hi[2], lo[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) hi[j] = s_q[(x * NB + b + j) * 64 + lane], lo[j] = s_q[(x * NB + b + j) * 64 + 32 + lane];
+#pragma unroll
+                    for (int s = 0; s < SL; ++s) {
+                        // two groups side by side, so that their sums' chains overlap; the small parts first
+                        float part[2][4];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) mma16816_first(part[j], ka[s][j][0], ka[s][j][1], ka[s][j][2], ka[s][j][3], lo[j].x, lo[j].y);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) mma16816(part[j], ka[s][j][4], ka[s][j][5], ka[s][j][6], ka[s][j][7], lo[j].z, lo[j].w);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) mma16816(part[j], ka[s][j][0], ka[s][j][1], ka[s][j][2], ka[s][j][3], hi[j].x, hi[j].y);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) mma16816(part[j], ka[s][j][4], ka[s][j][5], ka[s][j][6], ka[s][j][7], hi[j].z, hi[j].w);
+                        const float2 f0 = __half22float2(u32_h2(dk[s][0][b / 2])), f1 = __half22float2(u32_h2(dk[s][1][b / 2]));
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const float d0 = j ? f0.y : f0.x, d1 = j ? f1.y : f1.x;
+                            sv[s][i][0] = fmaf(d0, part[j][0], sv[s][i][0]), sv[s][i][1] = fmaf(d0, part[j][1], sv[s][i][1]);
+                            sv[s][i][2] = fmaf(d1, part[j][2], sv[s][i][2]), sv[s][i][3] = fmaf(d1, part[j][3], sv[s][i][3]);
+                        }
+                    }
                 }
             }
-            float t0 = -INFINITY, t1 = -INFINITY;
+            if (base + kTileCells > lim_min) {
 #pragma unroll
-            for (int s = 0; s < NT; ++s) t0 = fmaxf(t0, fmaxf(sv[s][0], sv[s][2])), t1 = fmaxf(t1, fmaxf(sv[s][1], sv[s][3]));
+                for (int s = 0; s < SL; ++s) {
+                    const int cell = base + (sg * SL + s) * 16 + g;
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) t0 = fmaxf(t0, __shfl_xor_sync(kFull, t0, o)), t1 = fmaxf(t1, __shfl_xor_sync(kFull, t1, o));
-            if (g == 0) *reinterpret_cast<float2 *>(s_wmax + (it & 1) * 64 + wid * 8 + 2 * t) = make_float2(t0, t1);
+                    for (int i = 0; i < NW; ++i) {
+                        if (cell >= lim[i][0]) sv[s][i][0] = -INFINITY;
+                        if (cell >= lim[i][1]) sv[s][i][1] = -INFINITY;
+                        if (cell + 8 >= lim[i][0]) sv[s][i][2] = -INFINITY;
+                        if (cell + 8 >= lim[i][1]) sv[s][i][3] = -INFINITY;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                if (NT > 1 && x_first + i * SL >= n_blocks) break;
+                float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+                for (int s = 0; s < SL; ++s) t0 = fmaxf(t0, fmaxf(sv[s][i][0], sv[s][i][2])), t1 = fmaxf(t1, fmaxf(sv[s][i][1], sv[s][i][3]));
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) t0 = fmaxf(t0, __shfl_xor_sync(kFull, t0, o)), t1 = fmaxf(t1, __shfl_xor_sync(kFull, t1, o));
+                if (g == 0) *reinterpret_cast<float2 *>(s_wmax + ((it & 1) * 8 + sg) * G::kCols + (x_first + i * SL) * 8 + 2 * t) = make_float2(t0, t1);
+            }
         };
         // probabilities of tile `it`, in the second product's fragment order; the factor its outputs rescale the sums by
         auto weights = [&](int it, float & r0, float & r1) {
-            // lane (g, t) takes the maxima that the g-th of the column block's warps found
-            float2 v = *reinterpret_cast<const float2 *>(s_wmax + (it & 1) * 64 + ((g % (8 / NT)) * NT + nt) * 8 + 2 * t);
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) v.x = fmaxf(v.x, __shfl_xor_sync(kFull, v.x, o)), v.y = fmaxf(v.y, __shfl_xor_sync(kFull, v.y, o));
-            const float n0 = fmaxf(m0, v.x * sc0), n1 = fmaxf(m1, v.y * sc1);
-            const float f0 = n0 == -INFINITY ? 0.0f : n0, f1 = n1 == -INFINITY ? 0.0f : n1;
-            r0 = ex2(m0 - f0), r1 = ex2(m1 - f1);
-            m0 = n0, m1 = n1;
-            l0 *= r0, l1 *= r1;
-            if (NT > 1 && slab0 == 0 && g == 0) *reinterpret_cast<float2 *>(s_corr + (it & 1) * G::kCols + nt * 8 + 2 * t) = make_float2(r0, r1);
-            const float b0 = kPShift - f0, b1 = kPShift - f1;
+            for (int i = 0; i < NW; ++i) {
+                const int x = x_first + i * SL;
+                if (NT > 1 && x >= n_blocks) break;
+                // lane (g, t) takes the maxima that the g-th slab group found
+                float2 v = *reinterpret_cast<const float2 *>(s_wmax + ((it & 1) * 8 + g % G::kSlabGroups) * G::kCols + x * 8 + 2 * t);
 #pragma unroll
-            for (int s = 0; s < NT; ++s) {
-                const float e0 = ex2(fmaf(sv[s][0], sc0, b0)), e1 = ex2(fmaf(sv[s][1], sc1, b1));
-                const float e2 = ex2(fmaf(sv[s][2], sc0, b0)), e3 = ex2(fmaf(sv[s][3], sc1, b1));
-                l0 += e0 + e2, l1 += e1 + e3;
-                uint32_t h0, h1, q0, q1;
-                split2(e0, e1, h0, q0);
-                split2(e2, e3, h1, q1);
-                s_prob[(((it & 1) * 8 + slab0 + s) * NT + nt) * 32 + lane] =
-                    make_uint4(transpose8x8(h0), transpose8x8(h1), transpose8x8(q0), transpose8x8(q1));
+                for (int o = 4; o < 32; o <<= 1) v.x = fmaxf(v.x, __shfl_xor_sync(kFull, v.x, o)), v.y = fmaxf(v.y, __shfl_xor_sync(kFull, v.y, o));
+                const float n0 = fmaxf(mx[i][0], v.x * sc[i][0]), n1 = fmaxf(mx[i][1], v.y * sc[i][1]);
+                const float f0 = n0 == -INFINITY ? 0.0f : n0, f1 = n1 == -INFINITY ? 0.0f : n1;
+                r0 = ex2(mx[i][0] - f0), r1 = ex2(mx[i][1] - f1);
+                mx[i][0] = n0, mx[i][1] = n1;
+                ls[i][0] *= r0, ls[i][1] *= r1;
+                if (NT > 1 && sg == 0 && g == 0) *reinterpret_cast<float2 *>(s_corr + (it & 1) * G::kCols + x * 8 + 2 * t) = make_float2(r0, r1);
+                const float b0 = kPShift - f0, b1 = kPShift - f1;
+#pragma unroll
+                for (int s = 0; s < SL; ++s) {
+                    const float e0 = ex2(fmaf(sv[s][i][0], sc[i][0], b0)), e1 = ex2(fmaf(sv[s][i][1], sc[i][1], b1));
+                    const float e2 = ex2(fmaf(sv[s][i][2], sc[i][0], b0)), e3 = ex2(fmaf(sv[s][i][3], sc[i][1], b1));
+                    ls[i][0] += e0 + e2, ls[i][1] += e1 + e3;
+                    uint32_t h0, h1, q0, q1;
+                    split2(e0, e1, h0, q0);
+                    split2(e2, e3, h1, q1);
+                    s_prob[(((it & 1) * 8 + sg * SL + s) * NT + x) * 32 + lane] =
+                        make_uint4(transpose8x8(h0), transpose8x8(h1), transpose8x8(q0), transpose8x8(q1));
+                }
             }
         };
         // tile `it`'s share of the outputs
@@ -614,6 +650,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             constexpr int NH = NT > 4 ? 4 : NT;                 // column blocks at a time (registers)
 #pragma unroll
             for (int x0 = 0; x0 < NT; x0 += NH) {
+                if (NT > 1 && x0 >= n_blocks) break;
                 float part[NH][2][4], small[NH == 1 ? 2 : 1][4];
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
@@ -628,7 +665,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                     uint32_t w[4];  // cells 0-7 and 8-15 of the first slab, then of the second
                     ldm4t(w, v_addr + sp * 16 * (HD / 2));
                     // a 256-wide cell's scales are a matrix row: transposed, lane (g, t) has group g's of cells 2 t, 2 t + 1
-                    uint32_t ds[NB == 8 ? 4 : 1];
+                    [[maybe_unused]] uint32_t ds[NB == 8 ? 4 : 1];
                     if constexpr (NB == 8) ldm4t(ds, smem_u32(vt) + G::kCodeBytes + (sp * 16 + lane) * 16);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
@@ -646,6 +683,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                         const uint32_t b2 = times(code_low(z1, p.e1024), db), b3 = times(code_high(z1, p.e64), db);
 #pragma unroll
                         for (int x = 0; x < NH; ++x) {
+                            if (NT > 1 && x0 + x >= n_blocks) break;
                             const uint4 f = s_prob[(((it & 1) * 8 + cg * kSlabs + sp + j) * NT + x0 + x) * 32 + lane];
                             if constexpr (NH == 1) {
                                 mma16816(small[0], a0, a1, a2, a3, f.z, f.w);
@@ -661,6 +699,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                 }
 #pragma unroll
                 for (int x = 0; x < NH; ++x) {
+                    if (NT > 1 && x0 + x >= n_blocks) break;
                     float2 f = make_float2(r0, r1);
                     if (NT > 1) f = *reinterpret_cast<const float2 *>(s_corr + (it & 1) * G::kCols + (x0 + x) * 8 + 2 * t);
 #pragma unroll
@@ -717,10 +756,16 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
 
         // ---- the item's end: sums across the warps, cell groups joined, rows written or left to be folded
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) l0 += __shfl_xor_sync(kFull, l0, o), l1 += __shfl_xor_sync(kFull, l1, o);
-        if (g == 0) {
-            *reinterpret_cast<float2 *>(s_lsum + wid * 8 + 2 * t) = make_float2(l0, l1);
-            if (slab0 == 0) *reinterpret_cast<float2 *>(s_mfin + nt * 8 + 2 * t) = make_float2(m0, m1);
+        for (int i = 0; i < NW; ++i) {
+            const int x = x_first + i * SL;
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                ls[i][0] += __shfl_xor_sync(kFull, ls[i][0], o), ls[i][1] += __shfl_xor_sync(kFull, ls[i][1], o);
+            }
+            if (g == 0) {
+                *reinterpret_cast<float2 *>(s_lsum + sg * G::kCols + x * 8 + 2 * t) = make_float2(ls[i][0], ls[i][1]);
+                if (sg == 0) *reinterpret_cast<float2 *>(s_mfin + x * 8 + 2 * t) = make_float2(mx[i][0], mx[i][1]);
+            }
         }
         float4 * s_red = reinterpret_cast<float4 *>(smem + G::red);
         if (cg > 0) {
@@ -750,14 +795,15 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             for (int x = 0; x < NT; ++x) {
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
+                    if (NT > 1 && x >= n_blocks) continue;
                     const int col = x * 8 + 2 * t + z, i = row_of_col(col);
                     if (i >= c.x.m) continue;
                     float l = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < 8 / NT; ++w) l += s_lsum[(w * NT + x) * 8 + 2 * t + z];
+                    for (int w = 0; w < G::kSlabGroups; ++w) l += s_lsum[w * G::kCols + col];
                     float4 o = make_float4(acc[x][0][z], acc[x][0][z + 2], acc[x][1][z], acc[x][1][z + 2]);
                     if (whole) {
-                        const int64_t at = (int64_t(c.x.row0 + i) * p.n_q + c.h * p.group + (col0 + col) % p.group) * HD + dg * 32 + 4 * g;
+                        const int64_t at = (int64_t(c.x.row0 + i) * p.n_q + c.h * p.group + (col0 + col - i * p.group)) * HD + dg * 32 + 4 * g;
                         const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
                         o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
                         if (p.gate != nullptr) {
@@ -779,81 +825,110 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
 }
 
 // ---- the fold -----------------------------------------------------------------------------------------------------------
-// Block (i, col): if piece i + 1 is the second of an item's, the item's pieces are folded for one column:
-// weights 2^(m - max), accumulators and sums joined in the order of the pieces, eight warps taking every eighth piece.
-constexpr int kFoldWarps = 8;
+// One column, VEC float4 vectors of dims a block, the other threads split the pieces: weights 2^(m - max), accumulators
+// and sums joined in the order of the pieces.  LISTED: block k takes the k-th, (k + gridDim.x)-th .. of the cut items,
+// found by listing the pieces' marks (few items, each in many pieces: few blocks an item would leave most of the machine
+// idle).  Else block k looks at piece k + 1 alone, which costs one load where there is nothing to fold.
+constexpr int kFoldThreads = 256;
 constexpr int kMaxPieces = 2 * kSmCount;
-template <int HD, int NT>
-__global__ void __launch_bounds__(kFoldWarps * 32) attend_paged_fold_kernel(const paged_params p) {
-    constexpr int COLS = 8 * NT, V = HD / 128 > 0 ? HD / 128 : 1;   // float4 vectors of a lane
-    constexpr int LANES = HD / 4 < 32 ? HD / 4 : 32;
-    __shared__ float4 s_acc[kFoldWarps][HD / 4];
-    __shared__ float s_max[kFoldWarps], s_sum[kFoldWarps];
+template <int HD, int NT, int VEC, bool LISTED>
+__global__ void __launch_bounds__(kFoldThreads) attend_paged_fold_kernel(const __grid_constant__ paged_params p, const int pieces_all) {
+    constexpr int COLS = 8 * NT, SPLIT = kFoldThreads / VEC;
+    __shared__ float4 s_acc[SPLIT][VEC];
+    __shared__ float s_max[kFoldThreads / 32], s_sum[kFoldThreads / 32];
     __shared__ float s_weight[kMaxPieces], s_part[kMaxPieces];
+    __shared__ uint16_t s_cut[kMaxPieces];
+    __shared__ int s_count[2 * kFoldThreads / 32];
+    static_assert(kMaxPieces <= 2 * kFoldThreads, "two heads a thread");
     pdl_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, col = blockIdx.y;
     pdl_wait();
-    const int col = blockIdx.y;
-    const fold_head f = *reinterpret_cast<const fold_head *>(p.ws_head + int64_t(blockIdx.x + 1) * 8);
-    if (f.fold == 0) return;
-    const request x = load_request<COLS>(p, f.r, false);
-    const int row = (f.blk * COLS + col) / p.group;
-    if (row >= x.m) return;
-
-    // weights of the pieces, then one pass over their accumulators.  The pieces after the first hold the item from their
-    // start: slot 0; in the first it is the last: slot 1.
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, n = f.to - f.from + 1;
-    auto slot_of = [&](int j) { return (int64_t(f.from + j) * 2 + (j == 0 ? 1 : 0)) * COLS + col; };
-    float top = -INFINITY;
-    for (int j = threadIdx.x; j < n; j += kFoldWarps * 32) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.ws_ml + slot_of(j) * 2));
-        s_weight[j] = ml.x, s_part[j] = ml.y;
-        top = fmaxf(top, ml.x);
+    auto head_of = [&](int i) { return reinterpret_cast<const fold_head *>(p.ws_head + int64_t(i) * 8); };
+    int cuts = int(blockIdx.x) + 1;
+    if constexpr (LISTED) {
+    // the cut items, in the order of the pieces: a thread two marks, listed by their rank
+    bool cut[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int i = tid + j * kFoldThreads;
+        cut[j] = i > 0 && i < pieces_all && __ldcg(p.ws_mark + i) != 0;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-    if (lane == 0) s_max[wid] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kFoldWarps; ++w) top = fmaxf(top, s_max[w]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
-    for (int j = threadIdx.x; j < n; j += kFoldWarps * 32) {
-        const float w = ex2(s_weight[j] - base);
-        s_weight[j] = w;
-        sum = fmaf(s_part[j], w, sum);
+    for (int j = 0; j < 2; ++j) {
+        const uint32_t some = __ballot_sync(kFull, cut[j]);
+        if (lane == 0) s_count[j * (kFoldThreads / 32) + wid] = __popc(some);
+        if (j == 1) __syncthreads();
     }
+    int before = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-    if (lane == 0) s_sum[wid] = sum;
-    __syncthreads();
-    float4 acc[V];
+    for (int j = 0; j < 2; ++j) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (lane < LANES) {
-#pragma unroll 8
-        for (int j = wid; j < n; j += kFoldWarps) {
-            const float w = s_weight[j];
-            const float4 * src = reinterpret_cast<const float4 *>(p.ws_acc + slot_of(j) * HD) + lane;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float4 a = __ldcg(src + 32 * v);
-                acc[v].x = fmaf(a.x, w, acc[v].x), acc[v].y = fmaf(a.y, w, acc[v].y);
-                acc[v].z = fmaf(a.z, w, acc[v].z), acc[v].w = fmaf(a.w, w, acc[v].w);
+        for (int w = 0; w < kFoldThreads / 32; ++w) {
+            const int at = j * (kFoldThreads / 32) + w;
+            if (w == wid) {
+                const uint32_t some = __ballot_sync(kFull, cut[j]);
+                if (cut[j]) s_cut[before + __popc(some & ((1u << lane) - 1))] = uint16_t(tid + j * kFoldThreads);
             }
+            before += s_count[at];
+        }
+    }
+    cuts = before;
+    __syncthreads();
+    }
+    for (int k = blockIdx.x; k < cuts; k += gridDim.x) {
+        const fold_head f = *head_of(LISTED ? int(s_cut[k]) : k + 1);
+        if (!LISTED && f.fold == 0) return;
+        const request x = load_request<COLS>(p, f.r, false);
+        const int row = (f.blk * COLS + col) / p.group;
+        if (row >= x.m) continue;
+        // The pieces after the first hold the item from their start: slot 0; in the first it is the last: slot 1.
+        const int n = f.to - f.from + 1;
+        auto slot_of = [&](int j) { return (int64_t(f.from + j) * 2 + (j == 0 ? 1 : 0)) * COLS + col; };
+        float top = -INFINITY;
+        for (int j = tid; j < n; j += kFoldThreads) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.ws_ml + slot_of(j) * 2));
+            s_weight[j] = ml.x, s_part[j] = ml.y;
+            top = fmaxf(top, ml.x);
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) s_acc[wid][lane + 32 * v] = acc[v];
-    }
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= HD) return;
-    float a = 0.0f, s = 0.0f;
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+        if (lane == 0) s_max[wid] = top;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kFoldWarps; ++w) a += reinterpret_cast<const float *>(s_acc[w])[d], s += s_sum[w];
-    float y = s == 0.0f ? 0.0f : __fdiv_rn(a, s);
-    const int64_t at = (int64_t(x.row0 + row) * p.n_q + f.h * p.group + (f.blk * COLS + col) % p.group) * HD + d;
-    if (p.gate != nullptr) y = __fdiv_rn(y, 1.0f + expf(-__ldg(p.gate + at)));
-    p.out[at] = y;
+        for (int w = 0; w < kFoldThreads / 32; ++w) top = fmaxf(top, s_max[w]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+        for (int j = tid; j < n; j += kFoldThreads) {
+            const float w = ex2(s_weight[j] - base);
+            s_weight[j] = w;
+            sum = fmaf(s_part[j], w, sum);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+        if (lane == 0) s_sum[wid] = sum;
+        __syncthreads();
+        const int v = tid % VEC, part = tid / VEC;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int j = part; j < n; j += SPLIT) {
+            const float w = s_weight[j];
+            const float4 a = __ldcg(reinterpret_cast<const float4 *>(p.ws_acc + slot_of(j) * HD) + blockIdx.z * VEC + v);
+            acc.x = fmaf(a.x, w, acc.x), acc.y = fmaf(a.y, w, acc.y), acc.z = fmaf(a.z, w, acc.z), acc.w = fmaf(a.w, w, acc.w);
+        }
+        s_acc[part][v] = acc;
+        __syncthreads();
+        if (tid < VEC * 4) {
+            float a = 0.0f, s = 0.0f;
+            for (int o = 0; o < min(SPLIT, n); ++o) a += reinterpret_cast<const float *>(s_acc[o])[tid];
+#pragma unroll
+            for (int w = 0; w < kFoldThreads / 32; ++w) s += s_sum[w];
+            float y = s == 0.0f ? 0.0f : __fdiv_rn(a, s);
+            const int64_t at = (int64_t(x.row0 + row) * p.n_q + f.h * p.group + (f.blk * COLS + col - row * p.group)) * HD + blockIdx.z * VEC * 4 + tid;
+            if (p.gate != nullptr) y = __fdiv_rn(y, 1.0f + expf(-__ldg(p.gate + at)));
+            p.out[at] = y;
+        }
+        __syncthreads();
+    }
 }
 
 // ---- launch -------------------------------------------------------------------------------------------------------------
@@ -884,7 +959,7 @@ size_t paged_workspace(const fnb_attend_paged_args * a) {
     if (one_tile(a)) return 16;  // no item is longer than a unit: nothing to fold
     const int nt = column_blocks(a);
     const size_t grid = size_t(ctas_of(nt)), cols = size_t(8 * nt);
-    return grid * 2 * cols * (size_t(a->head_dim) + 2) * 4 + grid * 32;
+    return grid * 2 * cols * (size_t(a->head_dim) + 2) * 4 + grid * 48;
 }
 
 bool paged_shape_ok(const fnb_attend_paged_args * a) {
@@ -892,11 +967,22 @@ bool paged_shape_ok(const fnb_attend_paged_args * a) {
     if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return false;
     if (a->rows < 1 || a->n_req < 1 || a->n_req > kMaxReq || a->max_pages < 1 || a->max_rows < 0) return false;
     if (a->row_start == nullptr && a->rows < a->n_req) return false;
+    if (int64_t(a->rows) * a->n_q_heads > INT32_MAX) return false;
     if (a->n_q_heads < 1 || a->n_kv_heads < 1 || a->n_q_heads > 1024 || a->n_q_heads % a->n_kv_heads != 0) return false;
     if (a->page_size < 16 || a->page_size > (1 << 20) || (a->page_size & (a->page_size - 1)) != 0) return false;
     if (a->cache_slots < a->page_size || a->cache_slots > INT32_MAX || a->cache_slots % a->page_size != 0) return false;
     if (a->cache_slots * a->n_kv_heads > int64_t(UINT32_MAX)) return false;
     return true;
+}
+
+void launch_fold(void (*kernel)(paged_params, int), dim3 blocks, cudaStream_t s, const paged_params & p, int grid) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = blocks, cfg.blockDim = dim3(kFoldThreads), cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    (void) cudaLaunchKernelEx(&cfg, kernel, p, grid);
 }
 
 template <int HD, int NT>
@@ -908,19 +994,21 @@ int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStre
     if (fold) {
         uint8_t * ws = static_cast<uint8_t *>(a->workspace);
         p.ws_head = reinterpret_cast<int32_t *>(ws);
-        p.ws_acc = reinterpret_cast<float *>(ws + size_t(grid) * 32);
+        p.ws_mark = p.ws_head + size_t(grid) * 8;
+        p.ws_acc = reinterpret_cast<float *>(ws + size_t(grid) * 48);
         p.ws_ml = p.ws_acc + size_t(grid) * 2 * cols * HD;
     }
     launch_pdl(attend_paged_kernel<HD, NT>, grid, kThreadsC, geo<HD, NT>::total, s, p);
     if (cudaPeekAtLastError() != cudaSuccess) return FNB_LAUNCH_FAILED;
     if (fold) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(unsigned(grid - 1), unsigned(cols)), cfg.blockDim = dim3(kFoldWarps * 32), cfg.stream = s;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr, cfg.numAttrs = 1;
-        (void) cudaLaunchKernelEx(&cfg, attend_paged_fold_kernel<HD, NT>, static_cast<const paged_params>(p));
+        // Few items of a long table: list them.  (The number of items goes by max_rows, a hint; a wrong one costs time only.)
+        const int64_t blocks = (int64_t(a->max_rows > 0 ? a->max_rows : 1) * p.group + cols - 1) / int64_t(cols);
+        const int64_t items = int64_t(a->n_req) * a->n_kv_heads * blocks;
+        if (items <= 16 && p.cells_max >= 64 * kTileCells) {
+            launch_fold(attend_paged_fold_kernel<HD, NT, 8, true>, dim3(unsigned(items), unsigned(cols), HD / 32), s, p, grid);
+        } else {
+            launch_fold(attend_paged_fold_kernel<HD, NT, HD / 4, false>, dim3(unsigned(grid - 1), unsigned(cols), 1), s, p, grid);
+        }
     }
     return launch_status();
 }
