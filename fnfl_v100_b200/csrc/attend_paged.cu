@@ -77,7 +77,7 @@ struct geo {
     static constexpr int mfin = corr + 2 * kCols * 4;           // float [kCols]
     static constexpr int red = mfin + kCols * 4;                // float4: the other cell groups' accumulators
     static constexpr int scan = red + (kCellGroups - 1) * kGroups * 32 * kCols * 4;  // int64 [8]: sums; the piece's start
-    static constexpr int total = scan + 10 * 8 + 1024;          // + slack to align the base to 1024 bytes
+    static constexpr int total = scan + 12 * 8 + 1024;          // + slack to align the base to 1024 bytes
     static_assert(total * kCtas + 1024 * kCtas <= 233472, "shared memory of an SM");
 };
 
@@ -96,6 +96,7 @@ struct paged_params {
     int rows, n_req, max_pages, n_pages, page_shift, n_q, n_kv, group;
     float scale_log2;
     uint32_t e1024, e64;  // FP16 exponents, twice each (code_low, code_high)
+    bool whole;           // pieces begin where items do
 };
 
 // ---- small pieces -----------------------------------------------------------------------------------------------------
@@ -355,20 +356,33 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     }
     const uint32_t total = uint32_t(sum);
     const pieces cut(total, gridDim.x);
-    const uint32_t u0 = cut.start(blockIdx.x), u1 = cut.start(blockIdx.x + 1);
-    if (u0 < u1 && upto > int64_t(u0) && upto - mine <= int64_t(u0)) {  // one thread
-        int64_t base = upto - mine;
-        for (int j = 0; j < per; ++j) {
-            const int64_t units = units_of(p, load_request<G::kCols>(p, tid * per + j, false));
-            if (base + units > int64_t(u0)) {
-                s_start[0] = uint32_t(tid * per + j);
-                s_start[1] = u0 - uint32_t(base);
-                break;
+    uint32_t u0 = cut.start(blockIdx.x), u1 = cut.start(blockIdx.x + 1);
+    auto find = [&](uint32_t u, int slot) {  // one thread: the request that holds unit u, and the unit's place in it
+        if (u < total && upto > int64_t(u) && upto - mine <= int64_t(u)) {
+            int64_t base = upto - mine;
+            for (int j = 0; j < per; ++j) {
+                const int64_t units = units_of(p, load_request<G::kCols>(p, tid * per + j, false));
+                if (base + units > int64_t(u)) {
+                    s_start[slot] = uint32_t(tid * per + j);
+                    s_start[slot + 1] = u - uint32_t(base);
+                    break;
+                }
+                base += units;
             }
-            base += units;
+        }
+    };
+    find(u0, 0);
+    if (p.whole) find(u1, 2);
+    __syncthreads();
+    if (p.whole && u0 < u1) {
+        cursor<G::kCols> at;
+        at.at(p, int(s_start[0]), s_start[1]);
+        u0 -= uint32_t(at.tile);
+        if (u1 < total) {
+            at.at(p, int(s_start[2]), s_start[3]);
+            u1 -= uint32_t(at.tile);
         }
     }
-    __syncthreads();
     if (u0 >= u1) {
         if (tid == 0 && p.ws_head != nullptr) {
             reinterpret_cast<fold_head *>(p.ws_head + int64_t(blockIdx.x) * 8)->fold = 0;
@@ -378,6 +392,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     }
     cursor<G::kCols> c;
     c.at(p, int(s_start[0]), s_start[1]);
+    if (p.whole) c.tile = 0;
     const uint32_t ring = smem_u32(smem) + G::ring;
     loader<HD, NT> load;
     load.start(p, c, u1 - u0);
@@ -954,9 +969,12 @@ int column_blocks(const fnb_attend_paged_args * a) {
     return cols <= 8 ? 1 : cols <= 16 ? 2 : cols <= 32 ? 4 : 8;
 }
 int ctas_of(int nt) { return kSmCount * (nt <= 2 ? 2 : 1); }
-bool one_tile(const fnb_attend_paged_args * a) { return int64_t(a->max_pages) * a->page_size <= kTileCells; }
+// Items of a few tiles stay whole: a CTA takes them from end to end, and there is nothing to fold.  Cut, a short item's
+// tiles run side by side, but the fold costs what three tiles take (8 requests of up to 300 cells: XX us cut, YY whole).
+constexpr int kWholeTiles = 2;
+bool whole_items(const fnb_attend_paged_args * a) { return int64_t(a->max_pages) * a->page_size <= kWholeTiles * kTileCells; }
 size_t paged_workspace(const fnb_attend_paged_args * a) {
-    if (one_tile(a)) return 16;  // no item is longer than a unit: nothing to fold
+    if (whole_items(a)) return 16;  // none is used
     const int nt = column_blocks(a);
     const size_t grid = size_t(ctas_of(nt)), cols = size_t(8 * nt);
     return grid * 2 * cols * (size_t(a->head_dim) + 2) * 4 + grid * 48;
@@ -990,7 +1008,7 @@ int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStre
     if (!configure<HD, NT>()) return FNB_LAUNCH_FAILED;
     const int grid = ctas_of(NT);
     const size_t cols = 8 * NT;
-    const bool fold = !one_tile(a);
+    const bool fold = !p.whole;
     if (fold) {
         uint8_t * ws = static_cast<uint8_t *>(a->workspace);
         p.ws_head = reinterpret_cast<int32_t *>(ws);
@@ -1045,7 +1063,7 @@ extern "C" int32_t fnb_attend_paged_kv4(const fnb_attend_paged_args * a, void * 
     }
     if (!ok_ptr(a->table, 4) || !ok_ptr(a->n_cells, 4) || !ok_opt(a->row_start, 4) || !ok_opt(a->err, 4)) return FNB_REJECTED;
     if (!(a->scale > 0.0f) || !(a->scale < INFINITY)) return FNB_REJECTED;
-    if (!one_tile(a) && (!ok_ptr(a->workspace, 16) || a->workspace_bytes < paged_workspace(a))) return FNB_REJECTED;
+    if (!whole_items(a) && (!ok_ptr(a->workspace, 16) || a->workspace_bytes < paged_workspace(a))) return FNB_REJECTED;
     paged_params p = {};
     p.k_cache = static_cast<const uint8_t *>(a->k_cache), p.v_cache = static_cast<const uint8_t *>(a->v_cache);
     p.q = a->q, p.gate = a->gate, p.k_scale = a->k_scale, p.v_scale = a->v_scale;
@@ -1056,6 +1074,7 @@ extern "C" int32_t fnb_attend_paged_kv4(const fnb_attend_paged_args * a, void * 
     p.n_pages = int(a->cache_slots / a->page_size), p.page_shift = __builtin_ctz(unsigned(a->page_size));
     p.n_q = a->n_q_heads, p.n_kv = a->n_kv_heads, p.group = a->n_q_heads / a->n_kv_heads;
     p.scale_log2 = a->scale * kLog2eF;
+    p.whole = whole_items(a);
     p.e1024 = 0x64006400u, p.e64 = 0x54005400u;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->head_dim == 256) return launch_paged_hd<256>(a, p, s);

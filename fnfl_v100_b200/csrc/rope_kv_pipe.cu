@@ -6,11 +6,11 @@
 // its speed is how many bytes each SM keeps in flight and how few instructions a row costs.  With loads into
 // registers the first is tied to occupancy; with cp.async.bulk it is a shared-memory budget:
 //
-//   producer warps (2)  per tile of `tt` tokens: three bulk copies (the tile's Q, K and V rows are each one
-//                       contiguous run in HBM) into stage s, completion counted in bytes on full[s]; while they
-//                       fly the producers compute the tile's (cos, sin) pairs - the F32 angle chain pos * ts^i
-//                       and the exact sincos, a token per warp - and resolve the tokens' cache slots, then arrive
-//                       on full[s] themselves.
+//   producer warps (2 or 4)  one crew of two that share a tile's tokens, or several crews that take tiles in turn.  Per
+//                       tile of `tt` tokens: three bulk copies (the tile's Q, K and V rows are each one contiguous run in
+//                       HBM) into stage s, completion counted in bytes on full[s]; while they fly the tile's producers
+//                       compute its (cos, sin) pairs - the F32 angle chain pos * ts^i and the exact sincos, a token per
+//                       warp - and resolve the tokens' cache slots, then arrive on full[s] themselves.
 //   consumer warps (20) two groups of ten; tiles alternate between the groups so two tiles are in work while up to
 //                       two more are in flight.  A warp takes four head rows at a time, EIGHT LANES PER ROW: lane
 //                       `sub` of a row holds values 4 sub .. 4 sub + 3 of each of the row's 32-value blocks (one
@@ -39,15 +39,16 @@ namespace {
 #define FNB_ROPE_GROUP_WARPS 10
 #endif
 #ifndef FNB_ROPE_PRODUCERS
-#define FNB_ROPE_PRODUCERS 2
+#define FNB_ROPE_PRODUCERS 4
 #endif
 #ifndef FNB_ROPE_MAX_STAGES
 #define FNB_ROPE_MAX_STAGES 4
 #endif
+static_assert(FNB_ROPE_PRODUCERS == 4 && FNB_ROPE_MAX_STAGES == 4, "crews divide the stages evenly");
 constexpr int kGroups = FNB_ROPE_GROUPS;
 constexpr int kGroupWarps = FNB_ROPE_GROUP_WARPS;
 constexpr int kConsumerWarps = kGroups * kGroupWarps;
-constexpr int kProducerWarps = FNB_ROPE_PRODUCERS;  // a token's angles are one warp's work of ~1000 cycles latency
+constexpr int kProducerWarps = FNB_ROPE_PRODUCERS;
 constexpr int kThreads = (kConsumerWarps + kProducerWarps) * 32;
 constexpr int kSlotBytes = 288;    // a 272-byte cell, padded to 16
 constexpr int kMaxTile = 8;        // tokens per tile at most
@@ -57,6 +58,7 @@ struct pipe_shape {
     int stages;        // a multiple of kGroups
     int nbh;           // n_rot / 64: blocks between the halves of a rotary pair (0: no rotation)
     uint32_t rpt_inv;  // ceil(2^32 / rows per token), for r / rpt by multiply-high
+    int share, crews;  // producer warps that share a tile's tokens (1 or 2); groups of them (1, 2 or 4, at most `stages`)
 };
 
 __device__ __forceinline__ float4 mul4(float4 a, float s) {
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1) rope_kv_pipe_kernel(const rope_ke
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
-            mbar_init(&full[s], kProducerWarps);
+            mbar_init(&full[s], uint32_t(sh.share));
             mbar_init(&empty[s], kGroupWarps);
         }
         mbar_init_fence();
@@ -142,32 +144,25 @@ __global__ void __launch_bounds__(kThreads, 1) rope_kv_pipe_kernel(const rope_ke
 
     if (wid >= kConsumerWarps) {
         // ---------------- producers ----------------
-        // Warp 0 of the pair issues the tile's copies; both compute the angles and resolve the cache slot of their
-        // share of the tile's tokens (token tk belongs to warp tk % kProducerWarps), then arrive.
+        // The tile's producer issues its copies, computes its tokens' angles and resolves their cache slots, then arrives.
         const int pw = wid - kConsumerWarps;
         const uint64_t policy = l2_evict_first_policy();
-        int it = 0;
-        bool ok = true;
-        for (int64_t tile = blockIdx.x; tile < n_tiles; tile += gridDim.x, ++it) {
+        // A crew takes every crews-th tile and so has stages of its own: it waits for a stage's phases one after the other,
+        // which a parity alone can tell apart.
+        const int crews = sh.crews, share = sh.share, crew = pw >> (share - 1), member = pw & (share - 1);
+        int it = crew;
+        for (int64_t tile = blockIdx.x + int64_t(crew) * gridDim.x; tile < n_tiles; tile += int64_t(crews) * gridDim.x, it += crews) {
             const int s = it % stages;
             const uint32_t ph = uint32_t(it / stages) & 1u;
             const int64_t t0 = tile * tt;
             const int live = int(a.rows - t0 < tt ? a.rows - t0 : tt);
-            // positions and slots do not depend on the stage: fetch them before waiting for it
-            int32_t p_of[kMaxTile / kProducerWarps];
-            int64_t c_of[kMaxTile / kProducerWarps];
-#pragma unroll
-            for (int j = 0; j < kMaxTile / kProducerWarps; ++j) {
-                const int tk = pw + j * kProducerWarps;
-                p_of[j] = tk < live ? __ldg(a.pos + t0 + tk) : 0;
-                c_of[j] = tk < live && a.slots != nullptr ? int64_t(__ldg(a.slots + t0 + tk)) : int64_t(p_of[j]);
-            }
-            if (it >= stages && !mbar_wait(&empty[s], ph ^ 1u, a.err)) {
-                ok = false;
-                break;
-            }
+            // positions and slots do not depend on the stage: fetch them before waiting for it, a token a lane
+            const bool mine = lane < live && (lane & (share - 1)) == member;
+            const int32_t p_mine = mine ? __ldg(a.pos + t0 + lane) : 0;
+            const int64_t c_mine = mine && a.slots != nullptr ? int64_t(__ldg(a.slots + t0 + lane)) : int64_t(p_mine);
+            if (it >= stages && !mbar_wait(&empty[s], ph ^ 1u, a.err)) break;
             uint8_t * st = data + size_t(s) * stage_bytes;
-            if (pw == 0 && lane == 0) {
+            if (member == 0 && lane == 0) {
                 mbar_expect_tx(&full[s], uint32_t(live) * (q_tok + 2 * kv_tok));
                 if (n_q > 0) bulk_g2s(st, a.q + t0 * n_q * HD, uint32_t(live) * q_tok, &full[s], policy);
                 if (n_kv > 0) {
@@ -176,14 +171,12 @@ __global__ void __launch_bounds__(kThreads, 1) rope_kv_pipe_kernel(const rope_ke
                              policy);
                 }
             }
-#pragma unroll
-            for (int j = 0; j < kMaxTile / kProducerWarps; ++j) {
-                const int tk = pw + j * kProducerWarps;
-                if (tk >= live) break;
+            for (int tk = member; tk < live; tk += share) {
                 float2 * cs = cs_all + (size_t(s) * tt + tk) * (HD / 2);
                 // lane i walks the chain pos * ts^i: i multiplies to reach its first pair, 32 more for each further one
                 // (with position planes, n_rot is 64: lane i is pair i and reads its own plane's position)
-                float theta = float(a.planes != nullptr ? __ldg(a.planes + 4 * (t0 + tk) + rope_plane_of_pair(lane)) : p_of[j]);
+                const int32_t pos = __shfl_sync(kFull, p_mine, tk);
+                float theta = float(a.planes != nullptr ? __ldg(a.planes + 4 * (t0 + tk) + rope_plane_of_pair(lane)) : pos);
 #pragma unroll
                 for (int c = 0; c < 31; ++c) theta = c < lane ? __fmul_rn(theta, a.theta_scale) : theta;
                 for (int i = lane; i < half; i += 32) {
@@ -192,22 +185,17 @@ __global__ void __launch_bounds__(kThreads, 1) rope_kv_pipe_kernel(const rope_ke
                     cs[i] = make_float2(cn, sn);
                     for (int c = 0; c < 32; ++c) theta = __fmul_rn(theta, a.theta_scale);
                 }
-                if (lane == 0) {
-                    cell_of[s * tt + tk] = rope_slot_ok<F>(c_of[j], a.cache_slots, a.err, true) ? int32_t(c_of[j]) : -1;
-                }
             }
+            if (mine) cell_of[s * tt + lane] = rope_slot_ok<F>(c_mine, a.cache_slots, a.err, true) ? int32_t(c_mine) : -1;
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[s]);
         }
-        // The copying producer leaves last: every copy it issued into this CTA's shared memory has landed (bounded)
-        // before the CTA can exit and the memory be handed to another CTA.  After a normal run these waits pass at
-        // once; after a wait that gave up, here or in a consumer, they are what keeps the exit safe.
-        (void) ok;
-        if (pw == 0 && lane == 0) {
-            for (int j = 1; j <= stages && j <= it; ++j) {
-                const int its = it - j;
-                mbar_wait_landed(&full[its % stages], uint32_t(its / stages) & 1u);
-            }
+        // Every copy this producer issued into the CTA's shared memory has landed (bounded) before it leaves, so before the
+        // CTA can exit and the memory be handed to another CTA.  After a normal run these waits pass at once; after a wait
+        // that gave up, here or in a consumer, they are what keeps the exit safe.  (`it` is its first tile not issued; the
+        // tile before in the same stage landed before that stage was filled again.)
+        if (member == 0 && lane == 0) {
+            for (int j = it - crews; j >= 0 && j >= it - stages; j -= crews) mbar_wait_landed(&full[j % stages], uint32_t(j / stages) & 1u);
         }
         return;
     }
@@ -314,7 +302,8 @@ __global__ void __launch_bounds__(kThreads, 1) rope_kv_pipe_kernel(const rope_ke
                     const int64_t c = int64_t(hh) * a.cache_slots + cell;
                     st_stream(reinterpret_cast<vec *>(cache + c * (HD / 2)) + sub, reinterpret_cast<const vec *>(my_slot)[sub]);
                     uint16_t * scl = (kind == 1 ? a.k_scale : a.v_scale) + c * NJ;
-                    if (sub == 0) st_stream(reinterpret_cast<vec *>(scl), reinterpret_cast<const vec *>(my_slot)[8]);
+                    // (an ordinary store: neighbouring slots' scales share 32-byte sectors, which L2 should gather)
+                    if (sub == 0) *reinterpret_cast<vec *>(scl) = reinterpret_cast<const vec *>(my_slot)[8];
                 }
                 __syncwarp();
                 continue;
@@ -410,8 +399,6 @@ bool launch_one(const rope_kernel_args & a, cudaStream_t s) {
     const int rpt = a.n_q + 2 * a.n_kv;
     if (rpt < 2) return false;  // r / rpt by multiply-high needs rpt >= 2
     const size_t tok_bytes = size_t(rpt) * HD * 4;
-    int tt = (kGroupWarps * 4) / rpt;  // one quad of rows per consumer warp and tile
-    tt = tt < 1 ? 1 : tt > kMaxTile ? kMaxTile : tt;
     const size_t fixed = size_t(3) * HD * 4 + size_t(kConsumerWarps) * 4 * kSlotBytes + 256;
     auto need = [&](int t, int st) {
         return size_t(st) * (size_t(t) * tok_bytes + size_t(t) * (HD / 2) * 8 + 16 + size_t(t) * 4) + fixed;
@@ -422,19 +409,29 @@ bool launch_one(const rope_kernel_args & a, cudaStream_t s) {
         while (st >= kGroups && need(t, st) > kSmemBudget) st -= kGroups;
         return st;
     };
-    int stages = fit(tt);
-    if (stages < kGroups && tt > 1) {
-        tt = 1;
-        stages = fit(tt);
+    // Tokens a tile: a group's warps take four rows each at a time, so the rows of a tile should fill whole rounds of them;
+    // of the sizes that do so best, among those that leave the ring its full depth, the smallest.
+    int tt = 1, stages = fit(1), best = 0;
+    for (int t = 1; t <= kMaxTile; ++t) {
+        const int st = fit(t), quads = (t * rpt + 3) / 4, rounds = (quads + kGroupWarps - 1) / kGroupWarps;
+        const int filled = t * rpt * 25 / (rounds * kGroupWarps);  // per cent
+        if (st == stages && filled > best + 2) tt = t, best = filled;
     }
     if (stages < kGroups) return false;
     const size_t smem = need(tt, stages);
 
     if (!ensure_configured<HD, F>()) return false;
+    // A token's angles are ~2500 cycles of dependent FP64 operations in one warp; the traffic of a token of 30 KB takes
+    // half of that.  Two warps keep up with such tokens (and more copies under way at once cost the 38 KB ones 6 %: 404
+    // against 428 us at 65 536 tokens of 16 + 2 + 2 heads of 256), four with smaller ones (8261 tokens of 8 + 8 + 8 heads of
+    // 128: 75 us with two, 36 with four).  Tiles of one token have nothing to share.
+    const int64_t token = int64_t(2 * a.n_q + 2 * a.n_kv) * HD * 4;
+    const int share = tt > 1 ? 2 : 1, warps = token >= 30000 ? 2 : kProducerWarps;
+    const int crews = warps / share < stages ? warps / share : stages;
     const int64_t n_tiles = (a.rows + tt - 1) / tt;
     const int grid = int(n_tiles < kSmCount ? n_tiles : kSmCount);
-    const pipe_shape sh{tt, stages, nbh, uint32_t((0x100000000ull + uint64_t(rpt) - 1) / uint64_t(rpt))};
-    launch_pdl(rope_kv_pipe_kernel<HD, F>, grid, kThreads, smem, s, a, sh);
+    const pipe_shape sh{tt, stages, nbh, uint32_t((0x100000000ull + uint64_t(rpt) - 1) / uint64_t(rpt)), share, crews};
+    launch_pdl(rope_kv_pipe_kernel<HD, F>, grid, (kConsumerWarps + crews * share) * 32, smem, s, a, sh);
     return true;
 }
 

@@ -43,6 +43,38 @@ def _same_device(*tensors) -> torch.device:
     return devs.pop()
 
 
+class _Here:
+    """The context of a call whose tensors live on the current device already."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on(first: torch.Tensor, *rest: torch.Tensor | None):
+    """_same_device and torch.cuda.device in one, for calls whose host time counts: two microseconds less where the
+    tensors' device is the current one.  `first` is known to be a CUDA tensor."""
+    d = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != d:
+            raise ValueError("tensors of one call must live on one CUDA device")
+    return _HERE if torch._C._cuda_getDevice() == d else torch.cuda.device(d)
+
+
+def _raw_stream(t: torch.Tensor) -> int:
+    """The current stream of t's device, without the Stream object torch.cuda.current_stream() makes (3 us)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _at(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
 def _numel(t: torch.Tensor | None, n: int, name: str) -> None:
     if t is not None and t.numel() != n:
         raise ValueError(f"{name}: expected {n} elements, got {t.numel()}")
@@ -244,9 +276,9 @@ def _rope_args(q, k, v, pos, slots, q_norm_w, k_norm_w, q_out, k_cache, v_cache,
             raise ValueError("planes: expected [rows][4]")
     cache_slots = k_cache.shape[0]
     a = _lib.RopeKvArgs(
-        _ptr(q).value, _ptr(k).value, _ptr(v).value, _ptr(pos).value, _ptr(slots).value, _ptr(q_norm_w).value,
-        _ptr(k_norm_w).value, _ptr(q_out).value, _ptr(k_cache).value, _ptr(v_cache).value, _ptr(k_f32).value,
-        _ptr(err).value, rows, cache_slots, n_q, k.shape[1], hd, n_rot, ts, eps, _ptr(planes).value)
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), _at(slots), _at(q_norm_w), _at(k_norm_w), q_out.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), _at(k_f32), _at(err), rows, cache_slots, n_q, k.shape[1], hd, n_rot, ts, eps,
+        _at(planes))
     return a
 
 
@@ -293,13 +325,6 @@ class PageTables(NamedTuple):
     free_head: torch.Tensor  # [1]
 
 
-def _out_i32(t: torch.Tensor | None, n: int, device, name: str) -> torch.Tensor:
-    if t is None:
-        return torch.empty(n, dtype=torch.int32, device=device)
-    _numel(_dev(t, torch.int32, name), n, name)
-    return t
-
-
 def page_tables(table: torch.Tensor, n_old: torch.Tensor, n_new: torch.Tensor, free_pages: torch.Tensor, *, page_size: int,
                 n_pages: int, rows: int, free_head: torch.Tensor | None = None, slots: torch.Tensor | None = None,
                 pos: torch.Tensor | None = None, row_start: torch.Tensor | None = None, n_cells: torch.Tensor | None = None,
@@ -317,24 +342,32 @@ def page_tables(table: torch.Tensor, n_old: torch.Tensor, n_new: torch.Tensor, f
     _dev(free_pages, torch.int32, "free_pages")
     if free_head is not None:
         _numel(_dev(free_head, torch.int32, "free_head"), 1, "free_head")
-    d = table.device
-    with torch.cuda.device(_same_device(table, n_old, n_new, free_pages, free_head, slots, pos, row_start, n_cells, free_head_out, _err(err))):
-        o = PageTables(_out_i32(slots, rows, d, "slots"), _out_i32(pos, rows, d, "pos"), _out_i32(row_start, n_req + 1, d, "row_start"),
-                       _out_i32(n_cells, n_req, d, "n_cells"), _out_i32(free_head_out, 1, d, "free_head_out"))
-        a = _lib.PageTablesArgs(n_old.data_ptr(), n_new.data_ptr(), free_pages.data_ptr(), _ptr(free_head).value, table.data_ptr(),
-                                o.n_cells.data_ptr(), o.row_start.data_ptr(), o.slots.data_ptr(), o.pos.data_ptr(),
-                                o.free_head.data_ptr(), _ptr(err).value, rows, free_pages.numel(), n_req, max_pages, n_pages, page_size)
-        _check(_lib.lib().fnb_page_tables(C.byref(a), _stream()), "page_tables")
-    return o
+    sizes = (rows, rows, n_req + 1, n_req, 1)
+    outs = [slots, pos, row_start, n_cells, free_head_out]
+    for i, name in enumerate(("slots", "pos", "row_start", "n_cells", "free_head_out")):
+        if outs[i] is not None:
+            _numel(_dev(outs[i], torch.int32, name), sizes[i], name)
+    with _on(table, n_old, n_new, free_pages, free_head, slots, pos, row_start, n_cells, free_head_out, _err(err)):
+        if rows > 0 and outs == [None] * 5:   # one allocation for all of them
+            outs = table.new_empty(2 * rows + 2 * n_req + 2).split_with_sizes(sizes)
+        else:
+            outs = [table.new_empty(n) if t is None else t for t, n in zip(outs, sizes)]
+        a = _lib.PageTablesArgs(n_old.data_ptr(), n_new.data_ptr(), free_pages.data_ptr(), _at(free_head), table.data_ptr(),
+                                outs[3].data_ptr(), outs[2].data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(), outs[4].data_ptr(),
+                                _at(err), rows, free_pages.numel(), n_req, max_pages, n_pages, page_size)
+        _check(_lib.lib().fnb_page_tables(C.byref(a), _raw_stream(table)), "page_tables")
+    return PageTables(*outs)
 
 
 def _kv4_planes(codes: torch.Tensor, scale: torch.Tensor, name: str) -> tuple[int, int, int]:
     """(n_kv, slots, head_dim) of a KV4 plane from new_kv_cache(fmt="kv4")."""
     _dev(codes, torch.uint8, name + "_cache")
     _dev(scale, torch.int16, name + "_scale")
-    if codes.dim() != 3 or tuple(scale.shape) != (codes.shape[0], codes.shape[1], codes.shape[2] // 16):
-        raise ValueError("%s_cache / %s_scale: expected the planes of new_kv_cache(fmt=\"kv4\")" % (name, name))
-    return codes.shape[0], codes.shape[1], codes.shape[2] * 2
+    if codes.dim() == 3:
+        n_kv, slots, row = codes.shape
+        if scale.shape == (n_kv, slots, row // 16):
+            return n_kv, slots, row * 2
+    raise ValueError("%s_cache / %s_scale: expected the planes of new_kv_cache(fmt=\"kv4\")" % (name, name))
 
 
 def rope_neox_kv4_append(q, k, v, pos, *, n_rot: int, theta_scale: float, k_cache, v_cache, k_scale, v_scale,
@@ -343,7 +376,7 @@ def rope_neox_kv4_append(q, k, v, pos, *, n_rot: int, theta_scale: float, k_cach
     """The norm + RoPE + append step into KV4 planes (new_kv_cache(fmt="kv4")): groups of 32 values as 4-bit codes and an
     FP16 scale.  A slot of -1 is a row of padding, for which nothing is written.  Returns q_out."""
     n_kv, n_slots, hd = _kv4_planes(k_cache, k_scale, "k")
-    if _kv4_planes(v_cache, v_scale, "v") != (n_kv, n_slots, hd) or tuple(k.shape[1:]) != (n_kv, hd):
+    if _kv4_planes(v_cache, v_scale, "v") != (n_kv, n_slots, hd) or k.shape[1:] != (n_kv, hd):
         raise ValueError("k_cache / v_cache: expected the planes of new_kv_cache for these heads")
     if q_out is None:
         q_out = torch.empty_like(q)
@@ -356,8 +389,8 @@ def rope_neox_kv4_append(q, k, v, pos, *, n_rot: int, theta_scale: float, k_cach
     base = _rope_args(q, k, v, pos, slots, q_norm_w, k_norm_w, q_out, k_cache, v_cache, k_f32, _err(err), n_rot, theta_scale, eps, planes)
     base.cache_slots = n_slots
     a = _lib.RopeKv8Args(base, k_scale.data_ptr(), v_scale.data_ptr())
-    with torch.cuda.device(_same_device(q, k, v, pos, slots, q_norm_w, k_norm_w, q_out, k_cache, v_cache, k_scale, v_scale, k_f32, err, planes)):
-        _check(_lib.lib().fnb_rope_neox_kv4_append(C.byref(a), _stream()), "rope_neox_kv4_append")
+    with _on(q, k, v, pos, slots, q_norm_w, k_norm_w, q_out, k_cache, v_cache, k_scale, v_scale, k_f32, err, planes):
+        _check(_lib.lib().fnb_rope_neox_kv4_append(C.byref(a), _raw_stream(q)), "rope_neox_kv4_append")
     return q_out
 
 
@@ -369,13 +402,17 @@ def kv4_read_f32(cache: torch.Tensor, scale: torch.Tensor, *, cells: torch.Tenso
         rows = _dev(cells, torch.int32, "cells").numel()
     elif rows is None:
         rows = slots - cell0
-    with torch.cuda.device(_same_device(cache, scale, cells, out, _err(err))):
+    with _on(cache, scale, cells, out, _err(err)):
         if out is None:
             out = torch.empty((rows, n_kv, hd), dtype=torch.float32, device=cache.device)
-        _numel(_dev(out, torch.float32, "out"), rows * n_kv * hd, "out")
-        a = _lib.KvReadArgs(cache.data_ptr(), scale.data_ptr(), _ptr(cells).value, out.data_ptr(), _ptr(err).value, rows, slots, cell0, n_kv, hd)
-        _check(_lib.lib().fnb_kv4_read_f32(C.byref(a), _stream()), "kv4_read_f32")
+        else:
+            _numel(_dev(out, torch.float32, "out"), rows * n_kv * hd, "out")
+        a = _lib.KvReadArgs(cache.data_ptr(), scale.data_ptr(), _at(cells), out.data_ptr(), _at(err), rows, slots, cell0, n_kv, hd)
+        _check(_lib.lib().fnb_kv4_read_f32(C.byref(a), _raw_stream(cache)), "kv4_read_f32")
     return out
+
+
+_NO_WORKSPACE = 16   # what fnb_attend_paged_workspace_bytes says for a call that uses none
 
 
 def attend_paged_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -399,22 +436,25 @@ def attend_paged_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         _numel(_dev(row_start, torch.int32, "row_start"), n_req + 1, "row_start")
     if gate is not None:
         _numel(_dev(gate, torch.float32, "gate"), q.numel(), "gate")
-    with torch.cuda.device(_same_device(q, k_cache, v_cache, k_scale, v_scale, table, n_cells, row_start, gate, out, workspace, _err(err))):
+    with _on(q, k_cache, v_cache, k_scale, v_scale, table, n_cells, row_start, gate, out, workspace, _err(err)):
         if out is None:
             out = torch.empty_like(q)
-        _numel(_dev(out, torch.float32, "out"), q.numel(), "out")
-        a = _lib.AttendPagedArgs(q.data_ptr(), _ptr(gate).value, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                                 v_scale.data_ptr(), table.data_ptr(), n_cells.data_ptr(), _ptr(row_start).value, out.data_ptr(), None, 0,
-                                 _ptr(err).value, slots, q.shape[0], n_req, max_pages, page_size, max_rows, q.shape[1], n_kv, hd,
+        else:
+            _numel(_dev(out, torch.float32, "out"), q.numel(), "out")
+        a = _lib.AttendPagedArgs(q.data_ptr(), _at(gate), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                 table.data_ptr(), n_cells.data_ptr(), _at(row_start), out.data_ptr(), None, 0, _at(err), slots,
+                                 q.shape[0], n_req, max_pages, page_size, max_rows, q.shape[1], n_kv, hd,
                                  hd ** -0.5 if scale is None else float(scale))
-        need = int(_lib.lib().fnb_attend_paged_workspace_bytes(C.byref(a)))
+        need = _lib.lib().fnb_attend_paged_workspace_bytes(C.byref(a))
         if need == 0:
             raise ValueError("attend_paged_kv4: shape outside the contract")
-        if workspace is None or workspace.numel() < need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _dev(workspace, torch.uint8, "workspace")
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-        _check(_lib.lib().fnb_attend_paged_kv4(C.byref(a), _stream()), "attend_paged_kv4")
+        if workspace is not None:
+            _dev(workspace, torch.uint8, "workspace")
+        if need > _NO_WORKSPACE:
+            if workspace is None or workspace.numel() < need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+        _check(_lib.lib().fnb_attend_paged_kv4(C.byref(a), _raw_stream(q)), "attend_paged_kv4")
     return out
 
 
