@@ -45,7 +45,6 @@
 namespace fnb {
 namespace {
 
-constexpr int kTileCells = 128;
 constexpr int kWarpsC = 8;
 constexpr int kThreadsC = kWarpsC * 32;
 constexpr int kMaxReq = 2048;
@@ -57,26 +56,33 @@ constexpr float kPShift = 14.0f;                 // probabilities are held times
 template <int HD, int NT>
 struct geo {
     static constexpr int kGroups = HD / 32;                     // scales of a cell; also 32-dim groups of the output
+    // cells of a tile: what a tile costs whatever its cells (the barrier, the walk, addresses) is the same for narrow heads
+    static constexpr int kTile = NT == 1 && HD < 256 ? 256 : 128, kSets = kTile / 128, kSlabs = kTile / 16;
     static constexpr int kCols = 8 * NT;
     static constexpr int kCellGroups = kWarpsC / kGroups;       // warps that share a dim group split the cells
-    static constexpr int kCodeBytes = kTileCells * HD / 2, kScaleBytes = kTileCells * kGroups * 2;
+    static constexpr int kCodeBytes = kTile * HD / 2, kScaleBytes = kTile * kGroups * 2;
     static constexpr int kUnitBytes = kCodeBytes + kScaleBytes;
     static constexpr int kCtas = NT <= 2 ? 2 : 1;               // resident on an SM (registers)
     // V is put out a tile behind K, so a third stage lets its copies begin a tile earlier; two where the memory is short
     static constexpr int kVStages = NT == 1 || NT == 4 ? 3 : 2, kStages = 2 + kVStages;   // K's stages, then V's
     // scores: a warp's slabs of 16 cells and column blocks.  With many columns two slabs share a fragment's load.
-    static constexpr int kSlabsW = NT >= 4 ? 2 : 1, kBlocksW = NT / kSlabsW, kSlabGroups = 8 / kSlabsW;
+    static constexpr int kShare = NT >= 4 ? 2 : 1;              // warps that split a slab group's column blocks
+    static constexpr int kSlabsW = kSets * kShare, kBlocksW = NT / kShare, kSlabGroups = 8 / kShare;
     static constexpr uint32_t kSwz = HD == 256 ? 7u : HD == 128 ? 3u : 1u;
     // shared memory
     static constexpr int ring = 0;
-    static constexpr int prob = ring + kStages * kUnitBytes;    // uint4 [2][8 slabs][NT][32]
-    static constexpr int qfrag = prob + 2 * 8 * NT * 512;       // uint4 [NT][kGroups][hi, lo][32]
+    static constexpr int prob = ring + kStages * kUnitBytes;    // uint4 [2][kSlabs][NT][32]
+    static constexpr int qfrag = prob + 2 * kSlabs * NT * 512;       // uint4 [NT][kGroups][hi, lo][32]
     static constexpr int wmax = qfrag + NT * kGroups * 1024;    // float [2][kSlabGroups][kCols]; and the queries' [kGroups][kCols]
     static constexpr int lsum = wmax + 2 * 8 * kCols * 4;       // float [kSlabGroups][kCols]
     static constexpr int corr = lsum + 8 * kCols * 4;           // float [2][kCols]
     static constexpr int mfin = corr + 2 * kCols * 4;           // float [kCols]
-    static constexpr int red = mfin + kCols * 4;                // float4: the other cell groups' accumulators
-    static constexpr int scan = red + (kCellGroups - 1) * kGroups * 32 * kCols * 4;  // int64 [8]: sums; the piece's start
+    // float4: the other cell groups' accumulators.  Of 128-wide heads they fit where the queries were: those are read up to
+    // the item's last scores, and the next item's are written behind a barrier of its own.
+    static constexpr int kRedBytes = (kCellGroups - 1) * kGroups * 32 * kCols * 4, tail = mfin + kCols * 4;
+    static constexpr bool kRedOnQueries = kRedBytes <= NT * kGroups * 1024;
+    static constexpr int red = kRedOnQueries ? qfrag : tail;
+    static constexpr int scan = tail + (kRedOnQueries ? 0 : kRedBytes);  // int64 [8]: sums; the piece's start
     static constexpr int total = scan + 12 * 8 + 1024;          // + slack to align the base to 1024 bytes
     static_assert(total * kCtas + 1024 * kCtas <= 233472, "shared memory of an SM");
 };
@@ -167,7 +173,7 @@ struct request {
     int n, m, row0;      // cells, rows, first row
     int tiles, blocks;   // of cells, of query columns
 };
-template <int COLS>
+template <class G>
 __device__ __forceinline__ request load_request(const paged_params & p, int r, bool report) {
     request x;
     int n = __ldg(p.n_cells + r);
@@ -180,8 +186,8 @@ __device__ __forceinline__ request load_request(const paged_params & p, int r, b
     x.row0 = x.row0 < 0 ? 0 : x.row0;
     end = end > p.rows ? p.rows : end;
     x.n = n, x.m = end > x.row0 ? end - x.row0 : 0;
-    x.tiles = n > 0 ? (n + kTileCells - 1) / kTileCells : 1;  // a request without cells still has rows to write
-    x.blocks = int((int64_t(x.m) * p.group + COLS - 1) / COLS);
+    x.tiles = n > 0 ? (n + G::kTile - 1) / G::kTile : 1;  // a request without cells still has rows to write
+    x.blocks = int((int64_t(x.m) * p.group + G::kCols - 1) / G::kCols);
     return x;
 }
 __device__ __forceinline__ int64_t units_of(const paged_params & p, const request & x) {
@@ -189,13 +195,13 @@ __device__ __forceinline__ int64_t units_of(const paged_params & p, const reques
 }
 
 // the walk over a piece of the line: request, KV head, column block, tile
-template <int COLS>
+template <class G>
 struct cursor {
     int r, h, blk, tile;
     request x;
     __device__ __forceinline__ void at(const paged_params & p, int request_index, uint32_t offset) {
         r = request_index;
-        x = load_request<COLS>(p, r, false);
+        x = load_request<G>(p, r, false);
         const uint32_t item = offset / uint32_t(x.tiles);
         tile = int(offset - item * uint32_t(x.tiles));
         h = int(item / uint32_t(x.blocks));
@@ -209,7 +215,7 @@ struct cursor {
         h = 0;
         do {
             if (++r >= p.n_req) return;
-            x = load_request<COLS>(p, r, false);
+            x = load_request<G>(p, r, false);
         } while (x.m == 0);
     }
 };
@@ -240,77 +246,109 @@ template <int HD, int NT>
 struct loader {
     using G = geo<HD, NT>;
     static constexpr int kCh = G::kGroups, kRows = 32 / kCh, kPass = 16 / kRows, kRow = HD / 2, kScale = kCh * 2;
-    static constexpr int kLag = 4 - G::kVStages;
-    cursor<G::kCols> c;
-    uint32_t step, tiles;  // of the piece
-    uint32_t v_stage;
-    int32_t id;            // page of the warp's rows in tile `step`
-    uint32_t cell[kLag];   // first of its rows in the kLag tiles before `step` (the last first), counted through all heads of a plane
-    int left[kLag];        // those tiles' cells from the warp's first row on
-    uint32_t lane_to;      // this lane's chunk of the warp's first pass within a stage
+    static constexpr int kLag = 4 - G::kVStages, S = G::kSets;  // a tile is S sets of 128 rows, sixteen to a warp
+    cursor<G> c;
+    uint32_t step, tiles;     // of the piece
+    uint32_t k_st, v_st;      // where the next copies go
+    int32_t id[S];            // pages of the warp's rows in tile `step`
+    uint32_t cell[kLag][S];   // first of its rows in the kLag tiles before `step` (the last first), counted through all heads of a plane
+    int left[kLag];           // those tiles' cells from the warp's first row on
+    uint32_t lane_to;         // this lane's chunk of the warp's first pass within a stage
 
     __device__ __forceinline__ static int warp_row() { return int(threadIdx.x >> 5) * 16; }
     __device__ __forceinline__ void fetch(const paged_params & p) {
-        const int at = c.tile * kTileCells + warp_row();
-        id = at < c.x.n ? __ldg(p.table + int64_t(c.r) * p.max_pages + (at >> p.page_shift)) : 0;
-    }
-    __device__ __forceinline__ void start(const paged_params & p, const cursor<G::kCols> & from, uint32_t n) {
-        c = from, step = 0, tiles = n, v_stage = 0;
+        const int32_t * t = p.table + int64_t(c.r) * p.max_pages;
 #pragma unroll
-        for (int i = 0; i < kLag; ++i) cell[i] = 0, left[i] = 0;
+        for (int q = 0; q < S; ++q) {
+            const int at = c.tile * G::kTile + q * 128 + warp_row();
+            id[q] = at < c.x.n ? __ldg(t + (at >> p.page_shift)) : 0;
+        }
+    }
+    __device__ __forceinline__ void start(const paged_params & p, const cursor<G> & from, uint32_t n, uint32_t ring) {
+        c = from, step = 0, tiles = n, k_st = ring, v_st = ring + 2 * G::kUnitBytes;
+#pragma unroll
+        for (int i = 0; i < kLag; ++i) {
+            left[i] = 0;
+#pragma unroll
+            for (int q = 0; q < S; ++q) cell[i][q] = 0;
+        }
         fetch(p);
         const uint32_t lane = threadIdx.x & 31, row = uint32_t(warp_row()) + lane / kCh;
         lane_to = row * kRow + (((lane % kCh) ^ ((row * kRow >> 7) & G::kSwz)) << 4);
     }
-    // `some` (at most sixteen count) of the rows at cell `first` into the stage at `st`
-    __device__ __forceinline__ void rows(const uint8_t * plane, uint32_t first, int some, uint32_t st) const {
+    // `some` (at most sixteen count) of the rows at cell `first` into set q of the stage at `st`
+    template <bool ALL>
+    __device__ __forceinline__ void rows(const uint8_t * plane, uint32_t first, int some, uint32_t st, int q) const {
         const uint32_t lane = threadIdx.x & 31;
         const uint8_t * src = plane + uint64_t(first) * kRow + lane * 16;
-        const uint32_t to = st + lane_to;
+        const uint32_t to = st + lane_to + q * 128 * kRow;
         // a 256-wide cell: four rows a pass, so every second pass has the other half of the eight row patterns
-        if (some >= 16) {
 #pragma unroll
-            for (int i = 0; i < kPass; ++i) copy_async<16>((to + i * kRows * kRow) ^ (kRows == 4 && (i & 1) ? 64u : 0u), src + i * kRows * kRow, true);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kPass; ++i) {
-                copy_async<16>((to + i * kRows * kRow) ^ (kRows == 4 && (i & 1) ? 64u : 0u), src + i * kRows * kRow, int(lane / kCh) + i * kRows < some);
-            }
+        for (int i = 0; i < kPass; ++i) {
+            copy_async<16>((to + i * kRows * kRow) ^ (kRows == 4 && (i & 1) ? 64u : 0u), src + i * kRows * kRow, ALL || int(lane / kCh) + i * kRows < some);
         }
+    }
+    // scales: the lower half-warp K's, the upper V's
+    template <bool ALL>
+    __device__ __forceinline__ void scales(const paged_params & p, uint32_t k_cell, uint32_t v_cell, int k_some, int v_some, int q) const {
+        const uint32_t lane = threadIdx.x & 31;
+        const bool lower = lane < 16;
+        const uint32_t at = (lower ? k_cell : v_cell) + (lane & 15);
+        copy_async<kScale>((lower ? k_st : v_st) + G::kCodeBytes + uint32_t(q * 128 + warp_row() + (lane & 15)) * kScale,
+                           (lower ? p.k_scale : p.v_scale) + uint64_t(at) * kCh, ALL || int(lane & 15) < (lower ? k_some : v_some));
     }
     __device__ __forceinline__ void next(const paged_params & p, uint32_t ring) {
         if (step >= tiles + kLag) return;
-        const uint32_t lane = threadIdx.x & 31;
         const bool k_too = step < tiles, v_too = step >= uint32_t(kLag);
-        const uint32_t k_st = ring + (step & 1) * G::kUnitBytes, v_st = ring + (2 + v_stage) * G::kUnitBytes;
-        const uint32_t v_cell = cell[kLag - 1];
-        const int v_left = left[kLag - 1];
-        if (v_too) rows(p.v_cache, v_cell, v_left, v_st);
+        const int base = c.tile * G::kTile + warp_row(), k_left = c.x.n - base, v_left = left[kLag - 1];
+        const uint32_t head = uint32_t(c.h) * uint32_t(p.cache_slots), mask = (1u << p.page_shift) - 1;
+        uint32_t k_cell[S];
+        bool known = true;
 #pragma unroll
-        for (int i = kLag - 1; i > 0; --i) cell[i] = cell[i - 1], left[i] = left[i - 1];
-        if (k_too) {
-            const int base = c.tile * kTileCells + warp_row();
-            left[0] = c.x.n - base;
-            if (uint32_t(id) >= uint32_t(p.n_pages)) {
-                if (lane == 0 && p.err != nullptr) atomicOr(p.err, FNB_ERR_PAGES);
-                id = 0;
-            }
-            cell[0] = uint32_t(c.h) * uint32_t(p.cache_slots) + (uint32_t(id) << p.page_shift) + (uint32_t(base) & ((1u << p.page_shift) - 1));
-            rows(p.k_cache, cell[0], left[0], k_st);
+        for (int q = 0; q < S; ++q) {
+            known = known && uint32_t(id[q]) < uint32_t(p.n_pages);
+            k_cell[q] = head + (uint32_t(id[q]) << p.page_shift) + (uint32_t(base + q * 128) & mask);
         }
-        const bool lower = lane < 16;
-        if (lower ? k_too : v_too) {
-            const uint32_t at = (lower ? cell[0] : v_cell) + (lane & 15);
-            copy_async<kScale>((lower ? k_st : v_st) + G::kCodeBytes + uint32_t(warp_row() + (lane & 15)) * kScale,
-                               (lower ? p.k_scale : p.v_scale) + uint64_t(at) * kCh, int(lane & 15) < (lower ? left[0] : v_left));
+        if (k_too && v_too && known && min(k_left, v_left) >= (S - 1) * 128 + 16) {
+#pragma unroll
+            for (int q = 0; q < S; ++q) {
+                rows<true>(p.v_cache, cell[kLag - 1][q], 16, v_st, q);
+                rows<true>(p.k_cache, k_cell[q], 16, k_st, q);
+                scales<true>(p, k_cell[q], cell[kLag - 1][q], 16, 16, q);
+            }
+        } else {
+            if (k_too && !known) {
+                if ((threadIdx.x & 31) == 0 && p.err != nullptr) atomicOr(p.err, FNB_ERR_PAGES);
+#pragma unroll
+                for (int q = 0; q < S; ++q) {
+                    if (uint32_t(id[q]) >= uint32_t(p.n_pages)) k_cell[q] = head + (uint32_t(base + q * 128) & mask);
+                }
+            }
+            const int k_all = k_too ? k_left : 0, v_all = v_too ? v_left : 0;
+#pragma unroll
+            for (int q = 0; q < S; ++q) {
+                if (v_too) rows<false>(p.v_cache, cell[kLag - 1][q], v_all - q * 128, v_st, q);
+                if (k_too) rows<false>(p.k_cache, k_cell[q], k_all - q * 128, k_st, q);
+                if ((threadIdx.x & 31) < 16 ? k_too : v_too) scales<false>(p, k_cell[q], cell[kLag - 1][q], k_all - q * 128, v_all - q * 128, q);
+            }
         }
         copies_commit();
+#pragma unroll
+        for (int i = kLag - 1; i > 0; --i) {
+            left[i] = left[i - 1];
+#pragma unroll
+            for (int q = 0; q < S; ++q) cell[i][q] = cell[i - 1][q];
+        }
+        left[0] = k_left;
+#pragma unroll
+        for (int q = 0; q < S; ++q) cell[0][q] = k_cell[q];
         if (step + 1 < tiles) {
             if (++c.tile >= c.x.tiles) c.next_item(p);
             fetch(p);
         }
         ++step;
-        if (v_too) v_stage = v_stage + 1 == G::kVStages ? 0 : v_stage + 1;
+        k_st = step & 1 ? ring + G::kUnitBytes : ring;
+        if (v_too) v_st = v_st == ring + (G::kStages - 1) * G::kUnitBytes ? ring + 2 * G::kUnitBytes : v_st + G::kUnitBytes;
     }
 };
 
@@ -334,7 +372,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     int64_t mine = 0;
     for (int j = 0; j < per; ++j) {
         const int r = tid * per + j;
-        if (r < p.n_req) mine += units_of(p, load_request<G::kCols>(p, r, blockIdx.x == 0));
+        if (r < p.n_req) mine += units_of(p, load_request<G>(p, r, blockIdx.x == 0));
     }
     int64_t upto = mine;
 #pragma unroll
@@ -361,7 +399,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         if (u < total && upto > int64_t(u) && upto - mine <= int64_t(u)) {
             int64_t base = upto - mine;
             for (int j = 0; j < per; ++j) {
-                const int64_t units = units_of(p, load_request<G::kCols>(p, tid * per + j, false));
+                const int64_t units = units_of(p, load_request<G>(p, tid * per + j, false));
                 if (base + units > int64_t(u)) {
                     s_start[slot] = uint32_t(tid * per + j);
                     s_start[slot + 1] = u - uint32_t(base);
@@ -375,7 +413,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     if (p.whole) find(u1, 2);
     __syncthreads();
     if (p.whole && u0 < u1) {
-        cursor<G::kCols> at;
+        cursor<G> at;
         at.at(p, int(s_start[0]), s_start[1]);
         u0 -= uint32_t(at.tile);
         if (u1 < total) {
@@ -390,12 +428,12 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         }
         return;
     }
-    cursor<G::kCols> c;
+    cursor<G> c;
     c.at(p, int(s_start[0]), s_start[1]);
     if (p.whole) c.tile = 0;
     const uint32_t ring = smem_u32(smem) + G::ring;
     loader<HD, NT> load;
-    load.start(p, c, u1 - u0);
+    load.start(p, c, u1 - u0, ring);
     if (tid == kThreadsC - 1 && p.ws_head != nullptr) {
         fold_head f = {0, 0, 0, c.r, c.h, c.blk};
         if (c.tile != 0) {
@@ -408,10 +446,10 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     }
 
     const int g = lane >> 2, t = lane & 3;
-    constexpr int SL = G::kSlabsW, NW = G::kBlocksW;
-    const int sg = wid / SL, x_first = wid % SL;                     // scores: slab group; column blocks x_first, + SL, ..
+    constexpr int SL = G::kSlabsW, NW = G::kBlocksW, SH = G::kShare;
+    const int sg = wid / SH, x_first = wid % SH;                     // scores: slab group; column blocks x_first, + SH, ..
     const int dg = wid % NB, cg = wid / NB;                          // outputs: dim group, cell group
-    constexpr int kSlabs = 8 / G::kCellGroups;                       // slabs of a cell group
+    constexpr int kSlabs = G::kSlabs / G::kCellGroups;                       // slabs of a cell group
     float * s_wmax = reinterpret_cast<float *>(smem + G::wmax);
     float * s_lsum = reinterpret_cast<float *>(smem + G::lsum);
     float * s_corr = reinterpret_cast<float *>(smem + G::corr);
@@ -425,7 +463,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     const uint32_t k_off = uint32_t(sg * SL * 16 + lrow) * (HD / 2) + ((uint32_t(lhalf) ^ swz) << 4);               // groups 0, 1
     const uint32_t v_off = uint32_t(cg * kSlabs * 16 + lhalf * 16 + lrow) * (HD / 2) + ((uint32_t(dg) ^ swz) << 4);  // slabs 0, 1
 
-    uint32_t k_stage = 0, v_stage = 0;  // of the next tile scored, of the next tile put out
+    uint32_t k_at = G::ring, v_at = G::ring + 2 * G::kUnitBytes;  // stages of the next tile scored, of the next tile put out
     uint32_t u = u0;
     while (u < u1) {
         const int tile_first = c.tile;
@@ -496,7 +534,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         for (int i = 0; i < NW; ++i) {
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
-                const int col = (x_first + i * SL) * 8 + 2 * t + z, r = row_of_col(col);
+                const int col = (x_first + i * SH) * 8 + 2 * t + z, r = row_of_col(col);
                 float up, down;
                 powers(top_of(col), up, down);
                 sc[i][z] = fmaxf(p.scale_log2 * down, 0x1p-126f);
@@ -521,10 +559,10 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
 
         // scores of tile `it` of the item into sv, their maxima to the other warps
         auto scores = [&](int it) {
-            const int base = (tile_first + it) * kTileCells;
-            const uint8_t * kt = smem + G::ring + k_stage * G::kUnitBytes;
-            const uint32_t k_addr = ring + k_stage * G::kUnitBytes + k_off;
-            k_stage ^= 1;
+            const int base = (tile_first + it) * G::kTile;
+            const uint8_t * kt = smem + k_at;
+            const uint32_t k_addr = smem_u32(smem) + k_at + k_off;
+            k_at = k_at == G::ring ? G::ring + G::kUnitBytes : G::ring;
             uint32_t dk[SL][2][NB / 2];
 #pragma unroll
             for (int s = 0; s < SL; ++s) {
@@ -560,7 +598,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                 }
 #pragma unroll
                 for (int i = 0; i < NW; ++i) {
-                    const int x = x_first + i * SL;
+                    const int x = x_first + i * SH;
                     if (NT > 1 && x >= n_blocks) break;
                     uint4 hi[2], lo[2];
 #pragma unroll
@@ -587,7 +625,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                     }
                 }
             }
-            if (base + kTileCells > lim_min) {
+            if (base + G::kTile > lim_min) {
 #pragma unroll
                 for (int s = 0; s < SL; ++s) {
                     const int cell = base + (sg * SL + s) * 16 + g;
@@ -602,20 +640,20 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             }
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
-                if (NT > 1 && x_first + i * SL >= n_blocks) break;
+                if (NT > 1 && x_first + i * SH >= n_blocks) break;
                 float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
                 for (int s = 0; s < SL; ++s) t0 = fmaxf(t0, fmaxf(sv[s][i][0], sv[s][i][2])), t1 = fmaxf(t1, fmaxf(sv[s][i][1], sv[s][i][3]));
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) t0 = fmaxf(t0, __shfl_xor_sync(kFull, t0, o)), t1 = fmaxf(t1, __shfl_xor_sync(kFull, t1, o));
-                if (g == 0) *reinterpret_cast<float2 *>(s_wmax + ((it & 1) * 8 + sg) * G::kCols + (x_first + i * SL) * 8 + 2 * t) = make_float2(t0, t1);
+                if (g == 0) *reinterpret_cast<float2 *>(s_wmax + ((it & 1) * 8 + sg) * G::kCols + (x_first + i * SH) * 8 + 2 * t) = make_float2(t0, t1);
             }
         };
         // probabilities of tile `it`, in the second product's fragment order; the factor its outputs rescale the sums by
         auto weights = [&](int it, float & r0, float & r1) {
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
-                const int x = x_first + i * SL;
+                const int x = x_first + i * SH;
                 if (NT > 1 && x >= n_blocks) break;
                 // lane (g, t) takes the maxima that the g-th slab group found
                 float2 v = *reinterpret_cast<const float2 *>(s_wmax + ((it & 1) * 8 + g % G::kSlabGroups) * G::kCols + x * 8 + 2 * t);
@@ -636,7 +674,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                     uint32_t h0, h1, q0, q1;
                     split2(e0, e1, h0, q0);
                     split2(e2, e3, h1, q1);
-                    s_prob[(((it & 1) * 8 + sg * SL + s) * NT + x) * 32 + lane] =
+                    s_prob[(((it & 1) * G::kSlabs + sg * SL + s) * NT + x) * 32 + lane] =
                         make_uint4(transpose8x8(h0), transpose8x8(h1), transpose8x8(q0), transpose8x8(q1));
                 }
             }
@@ -644,12 +682,13 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         // tile `it`'s share of the outputs
         auto outputs_of = [&](int it, float r0, float r1, auto some_masked) {
             constexpr bool masked = decltype(some_masked)::value;   // some row does not see some cell of the tile
-            const int base = (tile_first + it) * kTileCells;
-            uint8_t * vt = smem + G::ring + (2 + v_stage) * G::kUnitBytes;
-            const uint32_t v_addr = smem_u32(vt) + v_off;
-            v_stage = v_stage + 1 == G::kVStages ? 0 : v_stage + 1;
+            const int base = (tile_first + it) * G::kTile;
+            [[maybe_unused]] const uint32_t v_at_here = v_at;
+            uint8_t * vt = smem + v_at;
+            const uint32_t v_addr = smem_u32(smem) + v_at + v_off;
+            v_at = v_at == G::ring + (G::kStages - 1) * G::kUnitBytes ? G::ring + 2 * G::kUnitBytes : v_at + G::kUnitBytes;
             uint16_t * dv = reinterpret_cast<uint16_t *>(vt + G::kCodeBytes) + cg * kSlabs * 16 * NB + dg;  // this warp's cells and group
-            const int valid = masked ? min(kTileCells, c.x.n - base) - cg * kSlabs * 16 : kSlabs * 16;   // of its cells, those that were copied
+            const int valid = masked ? min(G::kTile, c.x.n - base) - cg * kSlabs * 16 : kSlabs * 16;   // of its cells, those that were copied
             uint32_t bad = 0;
             if constexpr (masked) {
                 // A cell that some row does not see may hold no number: this warp's scales of such cells become 0, and are
@@ -681,7 +720,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                     ldm4t(w, v_addr + sp * 16 * (HD / 2));
                     // a 256-wide cell's scales are a matrix row: transposed, lane (g, t) has group g's of cells 2 t, 2 t + 1
                     [[maybe_unused]] uint32_t ds[NB == 8 ? 4 : 1];
-                    if constexpr (NB == 8) ldm4t(ds, smem_u32(vt) + G::kCodeBytes + (sp * 16 + lane) * 16);
+                    if constexpr (NB == 8) ldm4t(ds, smem_u32(smem) + v_at_here + G::kCodeBytes + (sp * 16 + lane) * 16);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         __half2 da, db;  // scales of cells 2 t, 2 t + 1 and of 2 t + 8, 2 t + 9 of the slab
@@ -699,7 +738,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
 #pragma unroll
                         for (int x = 0; x < NH; ++x) {
                             if (NT > 1 && x0 + x >= n_blocks) break;
-                            const uint4 f = s_prob[(((it & 1) * 8 + cg * kSlabs + sp + j) * NT + x0 + x) * 32 + lane];
+                            const uint4 f = s_prob[(((it & 1) * G::kSlabs + cg * kSlabs + sp + j) * NT + x0 + x) * 32 + lane];
                             if constexpr (NH == 1) {
                                 mma16816(small[0], a0, a1, a2, a3, f.z, f.w);
                                 mma16816(small[NH == 1 ? 1 : 0], b0, b1, b2, b3, f.z, f.w);
@@ -744,7 +783,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         };
 
         auto outputs = [&](int it, float r0, float r1) {
-            if ((tile_first + it + 1) * kTileCells > lim_min) {
+            if ((tile_first + it + 1) * G::kTile > lim_min) {
                 outputs_of(it, r0, r1, std::true_type{});
             } else {
                 outputs_of(it, r0, r1, std::false_type{});
@@ -772,7 +811,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         // ---- the item's end: sums across the warps, cell groups joined, rows written or left to be folded
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-            const int x = x_first + i * SL;
+            const int x = x_first + i * SH;
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
                 ls[i][0] += __shfl_xor_sync(kFull, ls[i][0], o), ls[i][1] += __shfl_xor_sync(kFull, ls[i][1], o);
@@ -893,7 +932,7 @@ __global__ void __launch_bounds__(kFoldThreads) attend_paged_fold_kernel(const _
     for (int k = blockIdx.x; k < cuts; k += gridDim.x) {
         const fold_head f = *head_of(LISTED ? int(s_cut[k]) : k + 1);
         if (!LISTED && f.fold == 0) return;
-        const request x = load_request<COLS>(p, f.r, false);
+        const request x = load_request<geo<HD, NT>>(p, f.r, false);
         const int row = (f.blk * COLS + col) / p.group;
         if (row >= x.m) continue;
         // The pieces after the first hold the item from their start: slot 0; in the first it is the last: slot 1.
@@ -972,7 +1011,7 @@ int ctas_of(int nt) { return kSmCount * (nt <= 2 ? 2 : 1); }
 // Items of a few tiles stay whole: a CTA takes them from end to end, and there is nothing to fold.  Cut, a short item's
 // tiles run side by side, but the fold costs what three tiles take (8 requests of up to 300 cells: XX us cut, YY whole).
 constexpr int kWholeTiles = 2;
-bool whole_items(const fnb_attend_paged_args * a) { return int64_t(a->max_pages) * a->page_size <= kWholeTiles * kTileCells; }
+bool whole_items(const fnb_attend_paged_args * a) { return int64_t(a->max_pages) * a->page_size <= kWholeTiles * 128; }
 size_t paged_workspace(const fnb_attend_paged_args * a) {
     if (whole_items(a)) return 16;  // none is used
     const int nt = column_blocks(a);
@@ -1022,7 +1061,7 @@ int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStre
         // Few items of a long table: list them.  (The number of items goes by max_rows, a hint; a wrong one costs time only.)
         const int64_t blocks = (int64_t(a->max_rows > 0 ? a->max_rows : 1) * p.group + cols - 1) / int64_t(cols);
         const int64_t items = int64_t(a->n_req) * a->n_kv_heads * blocks;
-        if (items <= 16 && p.cells_max >= 64 * kTileCells) {
+        if (items <= 16 && p.cells_max >= 64 * 128) {
             launch_fold(attend_paged_fold_kernel<HD, NT, 8, true>, dim3(unsigned(items), unsigned(cols), HD / 32), s, p, grid);
         } else {
             launch_fold(attend_paged_fold_kernel<HD, NT, HD / 4, false>, dim3(unsigned(grid - 1), unsigned(cols), 1), s, p, grid);
@@ -1070,7 +1109,7 @@ extern "C" int32_t fnb_attend_paged_kv4(const fnb_attend_paged_args * a, void * 
     p.table = a->table, p.n_cells = a->n_cells, p.row_start = a->row_start, p.out = a->out, p.err = a->err;
     p.cache_slots = a->cache_slots, p.rows = a->rows, p.n_req = a->n_req, p.max_pages = a->max_pages;
     const int64_t held = int64_t(a->max_pages) * a->page_size;
-    p.cells_max = int(held < INT32_MAX - kTileCells ? held : INT32_MAX - kTileCells);
+    p.cells_max = int(held < INT32_MAX - 256 ? held : INT32_MAX - 256);
     p.n_pages = int(a->cache_slots / a->page_size), p.page_shift = __builtin_ctz(unsigned(a->page_size));
     p.n_q = a->n_q_heads, p.n_kv = a->n_kv_heads, p.group = a->n_q_heads / a->n_kv_heads;
     p.scale_log2 = a->scale * kLog2eF;
