@@ -45,36 +45,32 @@
 namespace fnb {
 namespace {
 
-constexpr int kWarpsC = 8;
-constexpr int kThreadsC = kWarpsC * 32;
 constexpr int kMaxReq = 2048;
 constexpr float kLog2eF = 1.4426950408889634f;
 constexpr float kPShift = 14.0f;                 // probabilities are held times 2^14
 
 // ---- geometry -------------------------------------------------------------------------------------------------------
-// HD: head_dim.  NT: blocks of eight query columns a unit serves (1, 2, 4 or 8).
+// HD: head_dim.  NT: blocks of eight query columns a unit serves (1, or 2 at 256).
 template <int HD, int NT>
 struct geo {
     static constexpr int kGroups = HD / 32;                     // scales of a cell; also 32-dim groups of the output
     // cells of a tile: what a tile costs whatever its cells (the barrier, the walk, addresses) is the same for narrow heads
     static constexpr int kTile = NT == 1 && HD < 256 ? 256 : 128, kSets = kTile / 128, kSlabs = kTile / 16;
     static constexpr int kCols = 8 * NT;
-    static constexpr int kCellGroups = kWarpsC / kGroups;       // warps that share a dim group split the cells
+    static constexpr int kWarps = 8, kThreads = kWarps * 32;
+    static constexpr int kCellGroups = 8 / kGroups;             // warps that share a dim group (and columns) split the cells
     static constexpr int kCodeBytes = kTile * HD / 2, kScaleBytes = kTile * kGroups * 2;
     static constexpr int kUnitBytes = kCodeBytes + kScaleBytes;
-    static constexpr int kCtas = NT <= 2 ? 2 : 1;               // resident on an SM (registers)
+    static constexpr int kCtas = 2;                             // resident on an SM (registers, shared memory)
     // V is put out a tile behind K, so a third stage lets its copies begin a tile earlier; two where the memory is short
-    static constexpr int kVStages = NT == 1 || NT == 4 ? 3 : 2, kStages = 2 + kVStages;   // K's stages, then V's
-    // scores: a warp's slabs of 16 cells and column blocks.  With many columns two slabs share a fragment's load.
-    static constexpr int kShare = NT >= 4 ? 2 : 1;              // warps that split a slab group's column blocks
-    static constexpr int kSlabsW = kSets * kShare, kBlocksW = NT / kShare, kSlabGroups = 8 / kShare;
+    static constexpr int kVStages = NT == 1 ? 3 : 2, kStages = 2 + kVStages;   // K's stages, then V's
     static constexpr uint32_t kSwz = HD == 256 ? 7u : HD == 128 ? 3u : 1u;
     // shared memory
     static constexpr int ring = 0;
     static constexpr int prob = ring + kStages * kUnitBytes;    // uint4 [2][kSlabs][NT][32]
     static constexpr int qfrag = prob + 2 * kSlabs * NT * 512;       // uint4 [NT][kGroups][hi, lo][32]
-    static constexpr int wmax = qfrag + NT * kGroups * 1024;    // float [2][kSlabGroups][kCols]; and the queries' [kGroups][kCols]
-    static constexpr int lsum = wmax + 2 * 8 * kCols * 4;       // float [kSlabGroups][kCols]
+    static constexpr int wmax = qfrag + NT * kGroups * 1024;    // float [2][kWarps][kCols]; and the queries' [kGroups][kCols]
+    static constexpr int lsum = wmax + 2 * 8 * kCols * 4;       // float [kWarps][kCols]
     static constexpr int corr = lsum + 8 * kCols * 4;           // float [2][kCols]
     static constexpr int mfin = corr + 2 * kCols * 4;           // float [kCols]
     // float4: the other cell groups' accumulators.  Of 128-wide heads they fit where the queries were: those are read up to
@@ -82,8 +78,8 @@ struct geo {
     static constexpr int kRedBytes = (kCellGroups - 1) * kGroups * 32 * kCols * 4, tail = mfin + kCols * 4;
     static constexpr bool kRedOnQueries = kRedBytes <= NT * kGroups * 1024;
     static constexpr int red = kRedOnQueries ? qfrag : tail;
-    static constexpr int scan = tail + (kRedOnQueries ? 0 : kRedBytes);  // int64 [8]: sums; the piece's start
-    static constexpr int total = scan + 12 * 8 + 1024;          // + slack to align the base to 1024 bytes
+    static constexpr int scan = tail + (kRedOnQueries ? 0 : kRedBytes);  // int64 [kWarps]: sums; the piece's start
+    static constexpr int total = scan + (kWarps + 4) * 8 + 1024;          // + slack to align the base to 1024 bytes
     static_assert(total * kCtas + 1024 * kCtas <= 233472, "shared memory of an SM");
 };
 
@@ -102,6 +98,9 @@ struct paged_params {
     int rows, n_req, max_pages, n_pages, page_shift, n_q, n_kv, group;
     float scale_log2;
     uint32_t e1024, e64;  // FP16 exponents, twice each (code_low, code_high)
+    // n / group = n group_mul >> group_shift for n < 2^31: group_mul = floor(2^(31 + l) / group) + 1 with 2^l >= group is off by
+    // at most group / 2^(31 + l) of 1 / group, so the product by less than 1 / group
+    uint32_t group_mul, group_shift;
     bool whole;           // pieces begin where items do
 };
 
@@ -149,6 +148,11 @@ __device__ __forceinline__ uint32_t code_high(uint32_t w, uint32_t e64) {
     return h2_u32(__hadd2(u32_h2((w & 0x00f000f0u) | e64), u32_h2(0xd480d480u)));    // - 72
 }
 __device__ __forceinline__ uint32_t times(uint32_t c, __half2 d) { return h2_u32(__hmul2(u32_h2(c), d)); }
+// infinities and NaN as 0
+__device__ __forceinline__ __half2 numbers_only(__half2 d) {
+    const uint32_t v = h2_u32(d);
+    return u32_h2(((v & 0x7c00u) == 0x7c00u ? 0u : v & 0xffffu) | ((v & 0x7c000000u) == 0x7c000000u ? 0u : v & 0xffff0000u));
+}
 // 2^x; results below 2^-126 are 0
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -354,21 +358,21 @@ struct loader {
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------
 template <int HD, int NT>
-__global__ void __launch_bounds__(kThreadsC, geo<HD, NT>::kCtas)
+__global__ void __launch_bounds__(geo<HD, NT>::kThreads, geo<HD, NT>::kCtas)
 attend_paged_kernel(const __grid_constant__ paged_params p) {
     using G = geo<HD, NT>;
     constexpr int NB = G::kGroups;
     extern __shared__ uint8_t smem_raw[];
     uint8_t * smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (rounding the pointer itself would make every access a generic one)
     int64_t * s_scan = reinterpret_cast<int64_t *>(smem + G::scan);
-    volatile uint32_t * s_start = reinterpret_cast<volatile uint32_t *>(s_scan + 8);  // the piece's first request, its unit there
+    volatile uint32_t * s_start = reinterpret_cast<volatile uint32_t *>(s_scan + G::kWarps);  // the piece's first request, its unit there
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
 
     pdl_launch_dependents();
     pdl_wait();
 
     // where this CTA's piece starts: sums of the requests' units, formed by every CTA for itself
-    const int per = (p.n_req + kThreadsC - 1) / kThreadsC;
+    const int per = (p.n_req + G::kThreads - 1) / G::kThreads;
     int64_t mine = 0;
     for (int j = 0; j < per; ++j) {
         const int r = tid * per + j;
@@ -384,7 +388,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     __syncthreads();
     int64_t sum = 0;
 #pragma unroll
-    for (int w = 0; w < kWarpsC; ++w) {
+    for (int w = 0; w < G::kWarps; ++w) {
         if (w < wid) upto += s_scan[w];
         sum += s_scan[w];
     }
@@ -434,7 +438,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     const uint32_t ring = smem_u32(smem) + G::ring;
     loader<HD, NT> load;
     load.start(p, c, u1 - u0, ring);
-    if (tid == kThreadsC - 1 && p.ws_head != nullptr) {
+    if (tid == G::kThreads - 1 && p.ws_head != nullptr) {
         fold_head f = {0, 0, 0, c.r, c.h, c.blk};
         if (c.tile != 0) {
             const uint32_t first = u0 - uint32_t(c.tile);          // the item's first unit
@@ -446,8 +450,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     }
 
     const int g = lane >> 2, t = lane & 3;
-    constexpr int SL = G::kSlabsW, NW = G::kBlocksW, SH = G::kShare;
-    const int sg = wid / SH, x_first = wid % SH;                     // scores: slab group; column blocks x_first, + SH, ..
+    constexpr int SL = G::kSets;                                     // scores: a warp's slabs of 16 cells, wid SL on
     const int dg = wid % NB, cg = wid / NB;                          // outputs: dim group, cell group
     constexpr int kSlabs = G::kSlabs / G::kCellGroups;                       // slabs of a cell group
     float * s_wmax = reinterpret_cast<float *>(smem + G::wmax);
@@ -460,7 +463,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     // (the same for every sixteenth row, so all addresses of a lane differ by constants)
     const int lrow = (lane & 7) + ((lane >> 3) & 1) * 8, lhalf = lane >> 4;
     const uint32_t swz = (uint32_t(lrow) * (HD / 2) >> 7) & G::kSwz;
-    const uint32_t k_off = uint32_t(sg * SL * 16 + lrow) * (HD / 2) + ((uint32_t(lhalf) ^ swz) << 4);               // groups 0, 1
+    const uint32_t k_off = uint32_t(wid * SL * 16 + lrow) * (HD / 2) + ((uint32_t(lhalf) ^ swz) << 4);               // groups 0, 1
     const uint32_t v_off = uint32_t(cg * kSlabs * 16 + lhalf * 16 + lrow) * (HD / 2) + ((uint32_t(dg) ^ swz) << 4);  // slabs 0, 1
 
     uint32_t k_at = G::ring, v_at = G::ring + 2 * G::kUnitBytes;  // stages of the next tile scored, of the next tile put out
@@ -470,7 +473,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         const int n_tiles = int(min(uint32_t(c.x.tiles - c.tile), u1 - u));
         const bool whole = tile_first == 0 && n_tiles == c.x.tiles;
         const int col0 = c.blk * G::kCols;
-        auto row_of_col = [&](int col) { return (col0 + col) / p.group; };
+        auto row_of_col = [&](int col) { return int(uint64_t(uint32_t(col0 + col)) * p.group_mul >> p.group_shift); };  // / p.group
 
         const int n_blocks = min(NT, (c.x.m * p.group - col0 + 7) / 8);   // column blocks with a live column
         // Queries, split, in the order of the fragments: lane (g, t) has dims 8 t + {0, 4}, {1, 5}, {2, 6}, {3, 7} of a group
@@ -499,8 +502,8 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         if (wid < kPairs) load8(wid % NB, wid / NB, first);
         if (load.step == 0) load.next(p, ring);              // the piece's first copies, while the queries arrive
 #pragma unroll
-        for (int k = 0; k * kWarpsC < kPairs; ++k) {
-            const int pair = wid + k * kWarpsC, b = pair % NB, x = pair / NB;
+        for (int k = 0; k * G::kWarps < kPairs; ++k) {
+            const int pair = wid + k * G::kWarps, b = pair % NB, x = pair / NB;
             if (pair >= kPairs) break;
             float4 v[2] = {first[0], first[1]};
             if (k > 0) load8(b, x, v);
@@ -511,10 +514,10 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             if (t == 0) s_wmax[b * G::kCols + x * 8 + g] = top;
         }
         if (load.step == 1) load.next(p, ring);
-        named_barrier<1>(kThreadsC);
+        named_barrier<1>(G::kThreads);
 #pragma unroll
-        for (int k = 0; k * kWarpsC < kPairs; ++k) {
-            const int pair = wid + k * kWarpsC, b = pair % NB, x = pair / NB;
+        for (int k = 0; k * G::kWarps < kPairs; ++k) {
+            const int pair = wid + k * G::kWarps, b = pair % NB, x = pair / NB;
             if (pair >= kPairs) break;
             float4 v[2] = {first[0], first[1]};
             if (k > 0) load8(b, x, v);                       // again, from L1
@@ -527,27 +530,27 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             split2(__fmul_rn(v[0].w, up), __fmul_rn(v[1].w, up), hi.w, lo.w);
             s_q[(x * NB + b) * 64 + lane] = hi, s_q[(x * NB + b) * 64 + 32 + lane] = lo;
         }
-        // this warp's columns: the factor of their scores, the cells they see; running maxima and sums
-        float sc[NW][2], mx[NW][2], ls[NW][2];
-        int lim[NW][2];
+        // columns 8 x + 2 t + z: the factor of their scores, the cells they see; running maxima, this warp's sums
+        float sc[NT][2], mx[NT][2], ls[NT][2];
+        int lim[NT][2];
 #pragma unroll
-        for (int i = 0; i < NW; ++i) {
+        for (int x = 0; x < NT; ++x) {
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
-                const int col = (x_first + i * SH) * 8 + 2 * t + z, r = row_of_col(col);
+                const int col = x * 8 + 2 * t + z, r = row_of_col(col);
                 float up, down;
                 powers(top_of(col), up, down);
-                sc[i][z] = fmaxf(p.scale_log2 * down, 0x1p-126f);
-                lim[i][z] = r < c.x.m ? c.x.n - c.x.m + r + 1 : 0;
-                mx[i][z] = -INFINITY, ls[i][z] = 0.0f;
+                sc[x][z] = fmaxf(p.scale_log2 * down, 0x1p-126f);
+                lim[x][z] = r < c.x.m ? c.x.n - c.x.m + r + 1 : 0;
+                mx[x][z] = -INFINITY, ls[x][z] = 0.0f;
             }
         }
         const int lim_min = c.x.n - c.x.m + row_of_col(0) + 1;   // cells every live row of the block sees
         copies_wait<1>();                                        // K of the piece's first tile
-        named_barrier<1>(kThreadsC);
+        named_barrier<1>(G::kThreads);
 
-        float sv[SL][NW][4];
-        float acc[NT][2][4];
+        float sv[SL][NT][4];
+        float acc[NT][2][4];  // column block x
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
 #pragma unroll
@@ -568,7 +571,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             for (int s = 0; s < SL; ++s) {
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
-                    const uint8_t * at = kt + G::kCodeBytes + ((sg * SL + s) * 16 + g + 8 * z) * (NB * 2);
+                    const uint8_t * at = kt + G::kCodeBytes + ((wid * SL + s) * 16 + g + 8 * z) * (NB * 2);
                     if constexpr (NB == 8) {
                         *reinterpret_cast<uint4 *>(dk[s][z]) = *reinterpret_cast<const uint4 *>(at);
                     } else if constexpr (NB == 4) {
@@ -578,7 +581,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < NW; ++i) sv[s][i][0] = sv[s][i][1] = sv[s][i][2] = sv[s][i][3] = 0.0f;
+                for (int x = 0; x < NT; ++x) sv[s][x][0] = sv[s][x][1] = sv[s][x][2] = sv[s][x][3] = 0.0f;
             }
 #pragma unroll
             for (int b = 0; b < NB; b += 2) {
@@ -589,16 +592,15 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                     ldm4(w, (k_addr + s * 16 * (HD / 2)) ^ uint32_t(b << 4));
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const uint32_t x0 = w[2 * j], x1 = w[2 * j + 1], y0 = x0 >> 8, y1 = x1 >> 8;
-                        ka[s][j][0] = code_low(x0, p.e1024), ka[s][j][1] = code_low(x1, p.e1024);
-                        ka[s][j][2] = code_high(x0, p.e64), ka[s][j][3] = code_high(x1, p.e64);
+                        const uint32_t w0 = w[2 * j], w1 = w[2 * j + 1], y0 = w0 >> 8, y1 = w1 >> 8;
+                        ka[s][j][0] = code_low(w0, p.e1024), ka[s][j][1] = code_low(w1, p.e1024);
+                        ka[s][j][2] = code_high(w0, p.e64), ka[s][j][3] = code_high(w1, p.e64);
                         ka[s][j][4] = code_low(y0, p.e1024), ka[s][j][5] = code_low(y1, p.e1024);
                         ka[s][j][6] = code_high(y0, p.e64), ka[s][j][7] = code_high(y1, p.e64);
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < NW; ++i) {
-                    const int x = x_first + i * SH;
+                for (int x = 0; x < NT; ++x) {
                     if (NT > 1 && x >= n_blocks) break;
                     uint4 hi[2], lo[2];
 #pragma unroll
@@ -618,9 +620,9 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                         const float2 f0 = __half22float2(u32_h2(dk[s][0][b / 2])), f1 = __half22float2(u32_h2(dk[s][1][b / 2]));
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            const float d0 = j ? f0.y : f0.x, d1 = j ? f1.y : f1.x;
-                            sv[s][i][0] = fmaf(d0, part[j][0], sv[s][i][0]), sv[s][i][1] = fmaf(d0, part[j][1], sv[s][i][1]);
-                            sv[s][i][2] = fmaf(d1, part[j][2], sv[s][i][2]), sv[s][i][3] = fmaf(d1, part[j][3], sv[s][i][3]);
+                            const float a = j ? f0.y : f0.x, c = j ? f1.y : f1.x;
+                            sv[s][x][0] = fmaf(a, part[j][0], sv[s][x][0]), sv[s][x][1] = fmaf(a, part[j][1], sv[s][x][1]);
+                            sv[s][x][2] = fmaf(c, part[j][2], sv[s][x][2]), sv[s][x][3] = fmaf(c, part[j][3], sv[s][x][3]);
                         }
                     }
                 }
@@ -628,53 +630,52 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             if (base + G::kTile > lim_min) {
 #pragma unroll
                 for (int s = 0; s < SL; ++s) {
-                    const int cell = base + (sg * SL + s) * 16 + g;
+                    const int cell = base + (wid * SL + s) * 16 + g;
 #pragma unroll
-                    for (int i = 0; i < NW; ++i) {
-                        if (cell >= lim[i][0]) sv[s][i][0] = -INFINITY;
-                        if (cell >= lim[i][1]) sv[s][i][1] = -INFINITY;
-                        if (cell + 8 >= lim[i][0]) sv[s][i][2] = -INFINITY;
-                        if (cell + 8 >= lim[i][1]) sv[s][i][3] = -INFINITY;
+                    for (int x = 0; x < NT; ++x) {
+                        if (cell >= lim[x][0]) sv[s][x][0] = -INFINITY;
+                        if (cell >= lim[x][1]) sv[s][x][1] = -INFINITY;
+                        if (cell + 8 >= lim[x][0]) sv[s][x][2] = -INFINITY;
+                        if (cell + 8 >= lim[x][1]) sv[s][x][3] = -INFINITY;
                     }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < NW; ++i) {
-                if (NT > 1 && x_first + i * SH >= n_blocks) break;
+            for (int x = 0; x < NT; ++x) {
+                if (NT > 1 && x >= n_blocks) break;
                 float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-                for (int s = 0; s < SL; ++s) t0 = fmaxf(t0, fmaxf(sv[s][i][0], sv[s][i][2])), t1 = fmaxf(t1, fmaxf(sv[s][i][1], sv[s][i][3]));
+                for (int s = 0; s < SL; ++s) t0 = fmaxf(t0, fmaxf(sv[s][x][0], sv[s][x][2])), t1 = fmaxf(t1, fmaxf(sv[s][x][1], sv[s][x][3]));
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) t0 = fmaxf(t0, __shfl_xor_sync(kFull, t0, o)), t1 = fmaxf(t1, __shfl_xor_sync(kFull, t1, o));
-                if (g == 0) *reinterpret_cast<float2 *>(s_wmax + ((it & 1) * 8 + sg) * G::kCols + (x_first + i * SH) * 8 + 2 * t) = make_float2(t0, t1);
+                if (g == 0) *reinterpret_cast<float2 *>(s_wmax + ((it & 1) * 8 + wid) * G::kCols + x * 8 + 2 * t) = make_float2(t0, t1);
             }
         };
         // probabilities of tile `it`, in the second product's fragment order; the factor its outputs rescale the sums by
         auto weights = [&](int it, float & r0, float & r1) {
 #pragma unroll
-            for (int i = 0; i < NW; ++i) {
-                const int x = x_first + i * SH;
+            for (int x = 0; x < NT; ++x) {
                 if (NT > 1 && x >= n_blocks) break;
-                // lane (g, t) takes the maxima that the g-th slab group found
-                float2 v = *reinterpret_cast<const float2 *>(s_wmax + ((it & 1) * 8 + g % G::kSlabGroups) * G::kCols + x * 8 + 2 * t);
+                // lane (g, t) takes the maxima that the g-th warp found
+                float2 v = *reinterpret_cast<const float2 *>(s_wmax + ((it & 1) * 8 + g) * G::kCols + x * 8 + 2 * t);
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) v.x = fmaxf(v.x, __shfl_xor_sync(kFull, v.x, o)), v.y = fmaxf(v.y, __shfl_xor_sync(kFull, v.y, o));
-                const float n0 = fmaxf(mx[i][0], v.x * sc[i][0]), n1 = fmaxf(mx[i][1], v.y * sc[i][1]);
+                const float n0 = fmaxf(mx[x][0], v.x * sc[x][0]), n1 = fmaxf(mx[x][1], v.y * sc[x][1]);
                 const float f0 = n0 == -INFINITY ? 0.0f : n0, f1 = n1 == -INFINITY ? 0.0f : n1;
-                r0 = ex2(mx[i][0] - f0), r1 = ex2(mx[i][1] - f1);
-                mx[i][0] = n0, mx[i][1] = n1;
-                ls[i][0] *= r0, ls[i][1] *= r1;
-                if (NT > 1 && sg == 0 && g == 0) *reinterpret_cast<float2 *>(s_corr + (it & 1) * G::kCols + x * 8 + 2 * t) = make_float2(r0, r1);
+                r0 = ex2(mx[x][0] - f0), r1 = ex2(mx[x][1] - f1);
+                mx[x][0] = n0, mx[x][1] = n1;
+                ls[x][0] *= r0, ls[x][1] *= r1;
+                if (NT > 1 && wid == 0 && g == 0) *reinterpret_cast<float2 *>(s_corr + (it & 1) * G::kCols + x * 8 + 2 * t) = make_float2(r0, r1);
                 const float b0 = kPShift - f0, b1 = kPShift - f1;
 #pragma unroll
                 for (int s = 0; s < SL; ++s) {
-                    const float e0 = ex2(fmaf(sv[s][i][0], sc[i][0], b0)), e1 = ex2(fmaf(sv[s][i][1], sc[i][1], b1));
-                    const float e2 = ex2(fmaf(sv[s][i][2], sc[i][0], b0)), e3 = ex2(fmaf(sv[s][i][3], sc[i][1], b1));
-                    ls[i][0] += e0 + e2, ls[i][1] += e1 + e3;
+                    const float e0 = ex2(fmaf(sv[s][x][0], sc[x][0], b0)), e1 = ex2(fmaf(sv[s][x][1], sc[x][1], b1));
+                    const float e2 = ex2(fmaf(sv[s][x][2], sc[x][0], b0)), e3 = ex2(fmaf(sv[s][x][3], sc[x][1], b1));
+                    ls[x][0] += e0 + e2, ls[x][1] += e1 + e3;
                     uint32_t h0, h1, q0, q1;
                     split2(e0, e1, h0, q0);
                     split2(e2, e3, h1, q1);
-                    s_prob[(((it & 1) * G::kSlabs + sg * SL + s) * NT + x) * 32 + lane] =
+                    s_prob[(((it & 1) * G::kSlabs + wid * SL + s) * NT + x) * 32 + lane] =
                         make_uint4(transpose8x8(h0), transpose8x8(h1), transpose8x8(q0), transpose8x8(q1));
                 }
             }
@@ -684,85 +685,78 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             constexpr bool masked = decltype(some_masked)::value;   // some row does not see some cell of the tile
             const int base = (tile_first + it) * G::kTile;
             [[maybe_unused]] const uint32_t v_at_here = v_at;
-            uint8_t * vt = smem + v_at;
+            const uint8_t * vt = smem + v_at;
             const uint32_t v_addr = smem_u32(smem) + v_at + v_off;
             v_at = v_at == G::ring + (G::kStages - 1) * G::kUnitBytes ? G::ring + 2 * G::kUnitBytes : v_at + G::kUnitBytes;
-            uint16_t * dv = reinterpret_cast<uint16_t *>(vt + G::kCodeBytes) + cg * kSlabs * 16 * NB + dg;  // this warp's cells and group
+            const uint16_t * dv = reinterpret_cast<const uint16_t *>(vt + G::kCodeBytes) + cg * kSlabs * 16 * NB + dg;  // this warp's cells and group
             const int valid = masked ? min(G::kTile, c.x.n - base) - cg * kSlabs * 16 : kSlabs * 16;   // of its cells, those that were copied
             uint32_t bad = 0;
             if constexpr (masked) {
-                // A cell that some row does not see may hold no number: this warp's scales of such cells become 0, and are
-                // put back below for the rows that see them.  (Behind the request's last cell all bytes are 0.)
+                // A cell that some row does not see may hold no number.  Its scale counts as 0 below, and the rows that do
+                // see it get their NaN back at the end.  (Behind the request's last cell all bytes are 0.)
 #pragma unroll
                 for (int j = 0; j < kSlabs / 2; ++j) {
-                    const int cell = lane + 32 * j;
-                    const bool none = (dv[cell * NB] & 0x7c00u) == 0x7c00u;
-                    if (none) bad |= 1u << j, dv[cell * NB] = 0;
+                    if ((dv[(lane + 32 * j) * NB] & 0x7c00u) == 0x7c00u) bad |= 1u << j;
                 }
-                __syncwarp();
             }
-            constexpr int NH = NT > 4 ? 4 : NT;                 // column blocks at a time (registers)
+            // the tile's sums: with one column block the small parts apart, which halves the chains
+            float part[NT][2][4], small[2][4];
 #pragma unroll
-            for (int x0 = 0; x0 < NT; x0 += NH) {
-                if (NT > 1 && x0 >= n_blocks) break;
-                float part[NH][2][4], small[NH == 1 ? 2 : 1][4];
+            for (int z = 0; z < 4; ++z) {
 #pragma unroll
-                for (int z = 0; z < 4; ++z) {
+                for (int x = 0; x < NT; ++x) part[x][0][z] = part[x][1][z] = 0.0f;
+                small[0][z] = small[1][z] = 0.0f;
+            }
 #pragma unroll
-                    for (int x = 0; x < NH; ++x) part[x][0][z] = part[x][1][z] = 0.0f;
-                    small[0][z] = 0.0f;
-                    if (NH == 1) small[NH == 1 ? 1 : 0][z] = 0.0f;
-                }
+            for (int sp = 0; sp < kSlabs; sp += 2) {
+                if (masked && sp * 16 >= valid) break;
+                uint32_t w[4];  // cells 0-7 and 8-15 of the first slab, then of the second
+                ldm4t(w, v_addr + sp * 16 * (HD / 2));
+                // a 256-wide cell's scales are a matrix row: transposed, lane (g, t) has group g's of cells 2 t, 2 t + 1
+                [[maybe_unused]] uint32_t ds[NB == 8 ? 4 : 1];
+                if constexpr (NB == 8) ldm4t(ds, smem_u32(smem) + v_at_here + G::kCodeBytes + (sp * 16 + lane) * 16);
 #pragma unroll
-                for (int sp = 0; sp < kSlabs; sp += 2) {
-                    if (masked && sp * 16 >= valid) break;
-                    uint32_t w[4];  // cells 0-7 and 8-15 of the first slab, then of the second
-                    ldm4t(w, v_addr + sp * 16 * (HD / 2));
-                    // a 256-wide cell's scales are a matrix row: transposed, lane (g, t) has group g's of cells 2 t, 2 t + 1
-                    [[maybe_unused]] uint32_t ds[NB == 8 ? 4 : 1];
-                    if constexpr (NB == 8) ldm4t(ds, smem_u32(smem) + v_at_here + G::kCodeBytes + (sp * 16 + lane) * 16);
+                for (int j = 0; j < 2; ++j) {
+                    __half2 da, db;  // scales of cells 2 t, 2 t + 1 and of 2 t + 8, 2 t + 9 of the slab
+                    if constexpr (NB == 8) {
+                        da = u32_h2(__shfl_sync(kFull, ds[2 * j], dg * 4 + t)), db = u32_h2(__shfl_sync(kFull, ds[2 * j + 1], dg * 4 + t));
+                    } else {
+                        const uint16_t * d = dv + ((sp + j) * 16 + 2 * t) * NB;
+                        da = u32_h2(uint32_t(d[0]) | (uint32_t(d[NB]) << 16)), db = u32_h2(uint32_t(d[8 * NB]) | (uint32_t(d[9 * NB]) << 16));
+                    }
+                    if constexpr (masked) da = numbers_only(da), db = numbers_only(db);
+                    const uint32_t y0 = w[2 * j], y1 = w[2 * j + 1], z0 = y0 >> 8, z1 = y1 >> 8;
+                    const uint32_t a0 = times(code_low(y0, p.e1024), da), a1 = times(code_high(y0, p.e64), da);
+                    const uint32_t a2 = times(code_low(y1, p.e1024), db), a3 = times(code_high(y1, p.e64), db);
+                    const uint32_t b0 = times(code_low(z0, p.e1024), da), b1 = times(code_high(z0, p.e64), da);
+                    const uint32_t b2 = times(code_low(z1, p.e1024), db), b3 = times(code_high(z1, p.e64), db);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        __half2 da, db;  // scales of cells 2 t, 2 t + 1 and of 2 t + 8, 2 t + 9 of the slab
-                        if constexpr (NB == 8) {
-                            da = u32_h2(__shfl_sync(kFull, ds[2 * j], dg * 4 + t)), db = u32_h2(__shfl_sync(kFull, ds[2 * j + 1], dg * 4 + t));
+                    for (int x = 0; x < NT; ++x) {
+                        if (NT > 1 && x >= n_blocks) break;
+                        const uint4 f = s_prob[(((it & 1) * G::kSlabs + cg * kSlabs + sp + j) * NT + x) * 32 + lane];
+                        if constexpr (NT == 1) {
+                            mma16816(small[0], a0, a1, a2, a3, f.z, f.w);
+                            mma16816(small[1], b0, b1, b2, b3, f.z, f.w);
                         } else {
-                            const uint16_t * d = dv + ((sp + j) * 16 + 2 * t) * NB;
-                            da = u32_h2(uint32_t(d[0]) | (uint32_t(d[NB]) << 16)), db = u32_h2(uint32_t(d[8 * NB]) | (uint32_t(d[9 * NB]) << 16));
+                            mma16816(part[x][0], a0, a1, a2, a3, f.z, f.w);
+                            mma16816(part[x][1], b0, b1, b2, b3, f.z, f.w);
                         }
-                        const uint32_t y0 = w[2 * j], y1 = w[2 * j + 1], z0 = y0 >> 8, z1 = y1 >> 8;
-                        const uint32_t a0 = times(code_low(y0, p.e1024), da), a1 = times(code_high(y0, p.e64), da);
-                        const uint32_t a2 = times(code_low(y1, p.e1024), db), a3 = times(code_high(y1, p.e64), db);
-                        const uint32_t b0 = times(code_low(z0, p.e1024), da), b1 = times(code_high(z0, p.e64), da);
-                        const uint32_t b2 = times(code_low(z1, p.e1024), db), b3 = times(code_high(z1, p.e64), db);
-#pragma unroll
-                        for (int x = 0; x < NH; ++x) {
-                            if (NT > 1 && x0 + x >= n_blocks) break;
-                            const uint4 f = s_prob[(((it & 1) * G::kSlabs + cg * kSlabs + sp + j) * NT + x0 + x) * 32 + lane];
-                            if constexpr (NH == 1) {
-                                mma16816(small[0], a0, a1, a2, a3, f.z, f.w);
-                                mma16816(small[NH == 1 ? 1 : 0], b0, b1, b2, b3, f.z, f.w);
-                            } else {
-                                mma16816(part[x][0], a0, a1, a2, a3, f.z, f.w);
-                                mma16816(part[x][1], b0, b1, b2, b3, f.z, f.w);
-                            }
-                            mma16816(part[x][0], a0, a1, a2, a3, f.x, f.y);
-                            mma16816(part[x][1], b0, b1, b2, b3, f.x, f.y);
-                        }
+                        mma16816(part[x][0], a0, a1, a2, a3, f.x, f.y);
+                        mma16816(part[x][1], b0, b1, b2, b3, f.x, f.y);
                     }
                 }
+            }
 #pragma unroll
-                for (int x = 0; x < NH; ++x) {
-                    if (NT > 1 && x0 + x >= n_blocks) break;
-                    float2 f = make_float2(r0, r1);
-                    if (NT > 1) f = *reinterpret_cast<const float2 *>(s_corr + (it & 1) * G::kCols + (x0 + x) * 8 + 2 * t);
+            for (int x = 0; x < NT; ++x) {
+                if (NT > 1 && x >= n_blocks) break;
+                float2 f = make_float2(r0, r1);
+                if (NT > 1) f = *reinterpret_cast<const float2 *>(s_corr + (it & 1) * G::kCols + x * 8 + 2 * t);
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
+                for (int y = 0; y < 2; ++y) {
 #pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const float add = NH == 1 ? part[x][y][z] + small[NH == 1 ? y : 0][z] : part[x][y][z];
-                            acc[x0 + x][y][z] = fmaf(acc[x0 + x][y][z], z & 1 ? f.y : f.x, add);
-                        }
+                    for (int z = 0; z < 4; ++z) {
+                        const float add = NT == 1 ? part[x][y][z] + small[y][z] : part[x][y][z];
+                        acc[x][y][z] = fmaf(acc[x][y][z], z & 1 ? f.y : f.x, add);
                     }
                 }
             }
@@ -796,7 +790,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         float r0 = 0.0f, r1 = 0.0f;
         for (int it = 0; it < n_tiles; ++it) {
             copies_wait<0>();
-            named_barrier<1>(kThreadsC);
+            named_barrier<1>(G::kThreads);
             load.next(p, ring);  // into the stages of this tile's K and of the V before the last
             float s0, s1;
             weights(it, s0, s1);
@@ -805,20 +799,19 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             r0 = s0, r1 = s1;
         }
         copies_wait<0>();
-        named_barrier<1>(kThreadsC);
+        named_barrier<1>(G::kThreads);
         outputs(n_tiles - 1, r0, r1);
 
         // ---- the item's end: sums across the warps, cell groups joined, rows written or left to be folded
 #pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            const int x = x_first + i * SH;
+        for (int x = 0; x < NT; ++x) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
-                ls[i][0] += __shfl_xor_sync(kFull, ls[i][0], o), ls[i][1] += __shfl_xor_sync(kFull, ls[i][1], o);
+                ls[x][0] += __shfl_xor_sync(kFull, ls[x][0], o), ls[x][1] += __shfl_xor_sync(kFull, ls[x][1], o);
             }
             if (g == 0) {
-                *reinterpret_cast<float2 *>(s_lsum + sg * G::kCols + x * 8 + 2 * t) = make_float2(ls[i][0], ls[i][1]);
-                if (sg == 0) *reinterpret_cast<float2 *>(s_mfin + x * 8 + 2 * t) = make_float2(mx[i][0], mx[i][1]);
+                *reinterpret_cast<float2 *>(s_lsum + wid * G::kCols + x * 8 + 2 * t) = make_float2(ls[x][0], ls[x][1]);
+                if (wid == 0) *reinterpret_cast<float2 *>(s_mfin + x * 8 + 2 * t) = make_float2(mx[x][0], mx[x][1]);
             }
         }
         float4 * s_red = reinterpret_cast<float4 *>(smem + G::red);
@@ -831,7 +824,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                 }
             }
         }
-        named_barrier<1>(kThreadsC);
+        named_barrier<1>(G::kThreads);
         if (cg == 0) {
 #pragma unroll
             for (int o = 1; o < G::kCellGroups; ++o) {
@@ -854,7 +847,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                     if (i >= c.x.m) continue;
                     float l = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < G::kSlabGroups; ++w) l += s_lsum[w * G::kCols + col];
+                    for (int w = 0; w < 8; ++w) l += s_lsum[w * G::kCols + col];
                     float4 o = make_float4(acc[x][0][z], acc[x][0][z + 2], acc[x][1][z], acc[x][1][z + 2]);
                     if (whole) {
                         const int64_t at = (int64_t(c.x.row0 + i) * p.n_q + c.h * p.group + (col0 + col - i * p.group)) * HD + dg * 32 + 4 * g;
@@ -1001,13 +994,16 @@ bool configure() {
     return true;
 }
 
-// Column blocks a unit serves: enough for a request of `max_rows` rows, so that its cells are read once; at most eight
-// (more rows are served by further passes over the cells).
+// Column blocks of eight a unit serves.  A 256-wide head's cells are read once for sixteen columns where a request has
+// that many; further columns are further passes.  (196 608 cells of 2 heads: two rows, 16 columns a head, 66 us against 75
+// in two passes; eight rows, 64 columns, 215 us against 231 and 270 with units of 32 and 64 columns, whose sums leave
+// registers for one CTA an SM.)  Narrow heads fare better with one block and the larger tiles it leaves room for (32
+// requests of up to 4096 cells, 8 heads of 128, eight rows of four: 92 us against 97).
 int column_blocks(const fnb_attend_paged_args * a) {
     const int64_t cols = int64_t(a->max_rows > 0 ? a->max_rows : 1) * (a->n_q_heads / a->n_kv_heads);
-    return cols <= 8 ? 1 : cols <= 16 ? 2 : cols <= 32 ? 4 : 8;
+    return a->head_dim == 256 && cols > 8 ? 2 : 1;
 }
-int ctas_of(int nt) { return kSmCount * (nt <= 2 ? 2 : 1); }
+constexpr int kGrid = 2 * kSmCount;  // two CTAs an SM
 // Items of a few tiles stay whole: a CTA takes them from end to end, and there is nothing to fold.  Cut, a short item's
 // tiles run side by side, but the fold costs what three tiles take (8 requests of up to 300 cells: XX us cut, YY whole).
 constexpr int kWholeTiles = 2;
@@ -1015,7 +1011,7 @@ bool whole_items(const fnb_attend_paged_args * a) { return int64_t(a->max_pages)
 size_t paged_workspace(const fnb_attend_paged_args * a) {
     if (whole_items(a)) return 16;  // none is used
     const int nt = column_blocks(a);
-    const size_t grid = size_t(ctas_of(nt)), cols = size_t(8 * nt);
+    const size_t grid = size_t(kGrid), cols = size_t(8 * nt);
     return grid * 2 * cols * (size_t(a->head_dim) + 2) * 4 + grid * 48;
 }
 
@@ -1045,7 +1041,7 @@ void launch_fold(void (*kernel)(paged_params, int), dim3 blocks, cudaStream_t s,
 template <int HD, int NT>
 int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStream_t s) {
     if (!configure<HD, NT>()) return FNB_LAUNCH_FAILED;
-    const int grid = ctas_of(NT);
+    const int grid = kGrid;
     const size_t cols = 8 * NT;
     const bool fold = !p.whole;
     if (fold) {
@@ -1055,37 +1051,26 @@ int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStre
         p.ws_acc = reinterpret_cast<float *>(ws + size_t(grid) * 48);
         p.ws_ml = p.ws_acc + size_t(grid) * 2 * cols * HD;
     }
-    launch_pdl(attend_paged_kernel<HD, NT>, grid, kThreadsC, geo<HD, NT>::total, s, p);
+    launch_pdl(attend_paged_kernel<HD, NT>, grid, geo<HD, NT>::kThreads, geo<HD, NT>::total, s, p);
     if (cudaPeekAtLastError() != cudaSuccess) return FNB_LAUNCH_FAILED;
     if (fold) {
         // Few items of a long table: list them.  (The number of items goes by max_rows, a hint; a wrong one costs time only.)
         const int64_t blocks = (int64_t(a->max_rows > 0 ? a->max_rows : 1) * p.group + cols - 1) / int64_t(cols);
         const int64_t items = int64_t(a->n_req) * a->n_kv_heads * blocks;
-        if (items <= 16 && p.cells_max >= 64 * 128) {
+        const int64_t outputs = items * int64_t(cols), wave = kSmCount * 8;   // columns to fold; blocks that run at a time
+        if (outputs * (HD / 32) <= wave && p.cells_max >= 64 * 128) {
             launch_fold(attend_paged_fold_kernel<HD, NT, 8, true>, dim3(unsigned(items), unsigned(cols), HD / 32), s, p, grid);
+        } else if (outputs <= wave && outputs < int64_t(grid - 1) * int64_t(cols) / 2 && p.cells_max >= 64 * 128) {
+            launch_fold(attend_paged_fold_kernel<HD, NT, HD / 4, true>, dim3(unsigned(items), unsigned(cols), 1), s, p, grid);
         } else {
             launch_fold(attend_paged_fold_kernel<HD, NT, HD / 4, false>, dim3(unsigned(grid - 1), unsigned(cols), 1), s, p, grid);
         }
     }
     return launch_status();
 }
-template <int HD>
-int32_t launch_paged_hd(const fnb_attend_paged_args * a, paged_params & p, cudaStream_t s) {
-    switch (column_blocks(a)) {
-        case 1: return launch_paged<HD, 1>(a, p, s);
-        case 2: return launch_paged<HD, 2>(a, p, s);
-        case 4: return launch_paged<HD, 4>(a, p, s);
-        default: return launch_paged<HD, 8>(a, p, s);
-    }
-}
-template <int HD>
-bool prepare_hd() { return configure<HD, 1>() && configure<HD, 2>() && configure<HD, 4>() && configure<HD, 8>(); }
-
 }  // namespace
 
-bool attend_paged_prepare_device() {
-    return prepare_hd<256>() && prepare_hd<128>() && prepare_hd<64>();
-}
+bool attend_paged_prepare_device() { return configure<256, 1>() && configure<256, 2>() && configure<128, 1>() && configure<64, 1>(); }
 
 }  // namespace fnb
 
@@ -1113,9 +1098,12 @@ extern "C" int32_t fnb_attend_paged_kv4(const fnb_attend_paged_args * a, void * 
     p.n_pages = int(a->cache_slots / a->page_size), p.page_shift = __builtin_ctz(unsigned(a->page_size));
     p.n_q = a->n_q_heads, p.n_kv = a->n_kv_heads, p.group = a->n_q_heads / a->n_kv_heads;
     p.scale_log2 = a->scale * kLog2eF;
+    int l = 0;
+    while ((1 << l) < p.group) ++l;
+    p.group_shift = 31 + l, p.group_mul = uint32_t((uint64_t(1) << p.group_shift) / uint64_t(p.group) + 1);
     p.whole = whole_items(a);
     p.e1024 = 0x64006400u, p.e64 = 0x54005400u;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a->head_dim == 256) return launch_paged_hd<256>(a, p, s);
-    return a->head_dim == 128 ? launch_paged_hd<128>(a, p, s) : launch_paged_hd<64>(a, p, s);
+    if (a->head_dim == 256) return column_blocks(a) == 2 ? launch_paged<256, 2>(a, p, s) : launch_paged<256, 1>(a, p, s);
+    return a->head_dim == 128 ? launch_paged<128, 1>(a, p, s) : launch_paged<64, 1>(a, p, s);
 }
