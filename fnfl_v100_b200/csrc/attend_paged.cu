@@ -23,19 +23,25 @@
 //   per group of 32 dims and outputs per tile in rounded F32 (sums run through all tiles in the tensor core were four
 //   times further from 64 bits).  Softmax statistics are F32.
 //
-// Work split: a unit is a tile of 128 cells of one (request, KV head, block of query columns).  The units of all
+// Work split: a unit is a tile of 128 cells (256 of narrow heads) of one (request, KV head, block of query columns).  The units of all
 // requests form one line that is cut into equal pieces, one for each resident CTA, wherever the requests' borders fall:
 // one long request and many ragged ones both fill the machine, from lengths only the device knows.  A piece that holds
 // all tiles of an item writes its rows itself; otherwise it leaves its sums, maximum and accumulators in the workspace
 // and a second launch folds an item's pieces in their order.  Results do not depend on timing.
 //
-// A CTA is eight warps.  Scores: a warp takes 16 cells for eight columns.  Maxima cross the warps through shared memory,
+// A CTA is eight warps.  Scores: a warp takes 16 cells (32) for eight columns.  Maxima cross the warps through shared memory,
 // probabilities go there in the order of the second product's fragments, and there a warp takes 32 dims of all cells.
 // Scores run a tile ahead of outputs, so one barrier a tile is enough: two K stages and three V stages, which every
 // thread fills for two tiles ahead with its share of 16-byte asynchronous copies, and each thread's wait for its own
-// copies before the barrier makes them everybody's.  Nothing else waits.  (Tensor-map copies, a page each, were tried
-// first: a page's four copies are issued one after another, by one warp that the seven others then wait for, or that
-// costs them registers as a ninth: 18 warps an SM put five on a scheduler.  61 us became XXX at 196 608 cells.)
+// copies before the barrier makes them everybody's (two V stages, and one tile ahead, for units of 16 columns).  Nothing
+// else waits.  (Tensor-map copies, a page each, were tried first: a page's four copies are issued one after another, by
+// one warp that the seven others then wait for, or that costs them registers as a ninth: 18 warps an SM put five on a
+// scheduler.  The change took 61 us to 50 at 196 608 cells.)
+//
+// Measured on a B200, graph replays over caches larger than L2: one request of 196 608 cells, 16 heads over 2 of 256:
+// 43.2 us, 113 MB at 2.6 TB/s; 40 requests of up to 8192 cells, 32 heads over 8 of 128: 58 us; 8 requests of up to 300
+// cells: 10.3 us, latency.  In its steady state a warp issues some 790 instructions a tile at 0.56 to 0.6 an issue slot,
+// the logic, FP16 and tensor units each 35 to 40 % busy; cells that lie in L2 give the same time.
 #include <atomic>
 #include <type_traits>
 
@@ -91,7 +97,6 @@ struct paged_params {
     float * out;
     float *ws_acc, *ws_ml;
     int32_t * ws_head;  // [grid][8]: what the fold has to do at the start of each piece (fold_head)
-    int32_t * ws_mark;  // [grid]: whether that is anything
     uint32_t * err;
     int64_t cache_slots;
     int cells_max;      // what a table row can list
@@ -237,8 +242,8 @@ struct pieces {
 
 // What the fold does at the start of a piece: nothing, or join the pieces `from` .. `to` of the item that was cut there
 // (only the first cut of an item says so).
-struct fold_head {
-    int32_t fold, from, to, r, h, blk;
+struct __align__(16) fold_head {
+    int32_t fold, from, to, h, blk, row0, m, unused;  // ..; head and column block of the item, its request's rows
 };
 
 // ---- the copies -------------------------------------------------------------------------------------------------------
@@ -428,7 +433,6 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     if (u0 >= u1) {
         if (tid == 0 && p.ws_head != nullptr) {
             reinterpret_cast<fold_head *>(p.ws_head + int64_t(blockIdx.x) * 8)->fold = 0;
-            p.ws_mark[blockIdx.x] = 0;
         }
         return;
     }
@@ -439,14 +443,13 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     loader<HD, NT> load;
     load.start(p, c, u1 - u0, ring);
     if (tid == G::kThreads - 1 && p.ws_head != nullptr) {
-        fold_head f = {0, 0, 0, c.r, c.h, c.blk};
+        fold_head f = {0, 0, 0, c.h, c.blk, c.x.row0, c.x.m, 0};
         if (c.tile != 0) {
             const uint32_t first = u0 - uint32_t(c.tile);          // the item's first unit
             f.from = int(cut.holder(first)), f.to = int(cut.holder(first + uint32_t(c.x.tiles) - 1));
             f.fold = int(blockIdx.x) == f.from + 1;                // a cut piece is never empty, so neither is the next
         }
         *reinterpret_cast<fold_head *>(p.ws_head + int64_t(blockIdx.x) * 8) = f;
-        p.ws_mark[blockIdx.x] = f.fold;
     }
 
     const int g = lane >> 2, t = lane & 3;
@@ -884,53 +887,60 @@ __global__ void __launch_bounds__(kFoldThreads) attend_paged_fold_kernel(const _
     __shared__ float4 s_acc[SPLIT][VEC];
     __shared__ float s_max[kFoldThreads / 32], s_sum[kFoldThreads / 32];
     __shared__ float s_weight[kMaxPieces], s_part[kMaxPieces];
-    __shared__ uint16_t s_cut[kMaxPieces];
+    __shared__ fold_head s_head[LISTED ? kMaxPieces : 1];
     __shared__ int s_count[2 * kFoldThreads / 32];
     static_assert(kMaxPieces <= 2 * kFoldThreads, "two heads a thread");
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, col = blockIdx.y;
     pdl_wait();
-    auto head_of = [&](int i) { return reinterpret_cast<const fold_head *>(p.ws_head + int64_t(i) * 8); };
+    auto head_of = [&](int i) {
+        const int4 * at = reinterpret_cast<const int4 *>(p.ws_head + int64_t(i) * 8);
+        const int4 a = __ldcg(at), b = __ldcg(at + 1);
+        return fold_head{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    };
     int cuts = int(blockIdx.x) + 1;
     if constexpr (LISTED) {
-    // the cut items, in the order of the pieces: a thread two marks, listed by their rank
-    bool cut[2];
+        // the cut items, in the order of the pieces: a thread two heads, listed by their rank among those that say so
+        fold_head head[2];
+        uint32_t some[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int i = tid + j * kFoldThreads;
-        cut[j] = i > 0 && i < pieces_all && __ldcg(p.ws_mark + i) != 0;
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const uint32_t some = __ballot_sync(kFull, cut[j]);
-        if (lane == 0) s_count[j * (kFoldThreads / 32) + wid] = __popc(some);
-        if (j == 1) __syncthreads();
-    }
-    int before = 0;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int w = 0; w < kFoldThreads / 32; ++w) {
-            const int at = j * (kFoldThreads / 32) + w;
-            if (w == wid) {
-                const uint32_t some = __ballot_sync(kFull, cut[j]);
-                if (cut[j]) s_cut[before + __popc(some & ((1u << lane) - 1))] = uint16_t(tid + j * kFoldThreads);
-            }
-            before += s_count[at];
+        for (int j = 0; j < 2; ++j) {
+            const int i = tid + j * kFoldThreads;
+            head[j].fold = 0;
+            if (i > 0 && i < pieces_all) head[j] = head_of(i);
         }
-    }
-    cuts = before;
-    __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            some[j] = __ballot_sync(kFull, head[j].fold != 0);
+            if (lane == 0) s_count[j * (kFoldThreads / 32) + wid] = __popc(some[j]);
+        }
+        __syncthreads();
+        cuts = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int w = 0; w < kFoldThreads / 32; ++w) {
+                if (w == wid && head[j].fold != 0) s_head[cuts + __popc(some[j] & ((1u << lane) - 1))] = head[j];
+                cuts += s_count[j * (kFoldThreads / 32) + w];
+            }
+        }
+        __syncthreads();
     }
     for (int k = blockIdx.x; k < cuts; k += gridDim.x) {
-        const fold_head f = *head_of(LISTED ? int(s_cut[k]) : k + 1);
+        const fold_head f = LISTED ? s_head[LISTED ? k : 0] : head_of(k + 1);
         if (!LISTED && f.fold == 0) return;
-        const request x = load_request<geo<HD, NT>>(p, f.r, false);
         const int row = (f.blk * COLS + col) / p.group;
-        if (row >= x.m) continue;
+        if (row >= f.m) continue;
         // The pieces after the first hold the item from their start: slot 0; in the first it is the last: slot 1.
         const int n = f.to - f.from + 1;
         auto slot_of = [&](int j) { return (int64_t(f.from + j) * 2 + (j == 0 ? 1 : 0)) * COLS + col; };
+        // the first pieces' accumulators are on their way before the weights are known
+        const int v = tid % VEC, part = tid / VEC;
+        auto acc_of = [&](int j) { return __ldcg(reinterpret_cast<const float4 *>(p.ws_acc + slot_of(j) * HD) + blockIdx.z * VEC + v); };
+        constexpr int kAhead = 4;
+        float4 ahead[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ahead[i] = part + i * SPLIT < n ? acc_of(part + i * SPLIT) : make_float4(0.f, 0.f, 0.f, 0.f);
         float top = -INFINITY;
         for (int j = tid; j < n; j += kFoldThreads) {
             const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.ws_ml + slot_of(j) * 2));
@@ -954,14 +964,16 @@ __global__ void __launch_bounds__(kFoldThreads) attend_paged_fold_kernel(const _
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
         if (lane == 0) s_sum[wid] = sum;
         __syncthreads();
-        const int v = tid % VEC, part = tid / VEC;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int j = part; j < n; j += SPLIT) {
-            const float w = s_weight[j];
-            const float4 a = __ldcg(reinterpret_cast<const float4 *>(p.ws_acc + slot_of(j) * HD) + blockIdx.z * VEC + v);
+        auto join = [&](float4 a, float w) {
             acc.x = fmaf(a.x, w, acc.x), acc.y = fmaf(a.y, w, acc.y), acc.z = fmaf(a.z, w, acc.z), acc.w = fmaf(a.w, w, acc.w);
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (part + i * SPLIT < n) join(ahead[i], s_weight[part + i * SPLIT]);
         }
+#pragma unroll 8
+        for (int j = part + kAhead * SPLIT; j < n; j += SPLIT) join(acc_of(j), s_weight[j]);
         s_acc[part][v] = acc;
         __syncthreads();
         if (tid < VEC * 4) {
@@ -970,7 +982,7 @@ __global__ void __launch_bounds__(kFoldThreads) attend_paged_fold_kernel(const _
 #pragma unroll
             for (int w = 0; w < kFoldThreads / 32; ++w) s += s_sum[w];
             float y = s == 0.0f ? 0.0f : __fdiv_rn(a, s);
-            const int64_t at = (int64_t(x.row0 + row) * p.n_q + f.h * p.group + (f.blk * COLS + col - row * p.group)) * HD + blockIdx.z * VEC * 4 + tid;
+            const int64_t at = (int64_t(f.row0 + row) * p.n_q + f.h * p.group + (f.blk * COLS + col - row * p.group)) * HD + blockIdx.z * VEC * 4 + tid;
             if (p.gate != nullptr) y = __fdiv_rn(y, 1.0f + expf(-__ldg(p.gate + at)));
             p.out[at] = y;
         }
@@ -1005,14 +1017,15 @@ int column_blocks(const fnb_attend_paged_args * a) {
 }
 constexpr int kGrid = 2 * kSmCount;  // two CTAs an SM
 // Items of a few tiles stay whole: a CTA takes them from end to end, and there is nothing to fold.  Cut, a short item's
-// tiles run side by side, but the fold costs what three tiles take (8 requests of up to 300 cells: XX us cut, YY whole).
+// tiles run side by side, and the fold costs less than three tiles in a row (8 requests of up to 300 cells, 16 heads over 2
+// of 256: 10.3 us cut, 11.9 whole).
 constexpr int kWholeTiles = 2;
 bool whole_items(const fnb_attend_paged_args * a) { return int64_t(a->max_pages) * a->page_size <= kWholeTiles * 128; }
 size_t paged_workspace(const fnb_attend_paged_args * a) {
     if (whole_items(a)) return 16;  // none is used
     const int nt = column_blocks(a);
     const size_t grid = size_t(kGrid), cols = size_t(8 * nt);
-    return grid * 2 * cols * (size_t(a->head_dim) + 2) * 4 + grid * 48;
+    return grid * 2 * cols * (size_t(a->head_dim) + 2) * 4 + grid * 32;
 }
 
 bool paged_shape_ok(const fnb_attend_paged_args * a) {
@@ -1047,8 +1060,7 @@ int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStre
     if (fold) {
         uint8_t * ws = static_cast<uint8_t *>(a->workspace);
         p.ws_head = reinterpret_cast<int32_t *>(ws);
-        p.ws_mark = p.ws_head + size_t(grid) * 8;
-        p.ws_acc = reinterpret_cast<float *>(ws + size_t(grid) * 48);
+        p.ws_acc = reinterpret_cast<float *>(ws + size_t(grid) * 32);
         p.ws_ml = p.ws_acc + size_t(grid) * 2 * cols * HD;
     }
     launch_pdl(attend_paged_kernel<HD, NT>, grid, geo<HD, NT>::kThreads, geo<HD, NT>::total, s, p);
@@ -1060,7 +1072,7 @@ int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStre
         const int64_t outputs = items * int64_t(cols), wave = kSmCount * 8;   // columns to fold; blocks that run at a time
         if (outputs * (HD / 32) <= wave && p.cells_max >= 64 * 128) {
             launch_fold(attend_paged_fold_kernel<HD, NT, 8, true>, dim3(unsigned(items), unsigned(cols), HD / 32), s, p, grid);
-        } else if (outputs <= wave && outputs < int64_t(grid - 1) * int64_t(cols) / 2 && p.cells_max >= 64 * 128) {
+        } else if (outputs <= wave) {
             launch_fold(attend_paged_fold_kernel<HD, NT, HD / 4, true>, dim3(unsigned(items), unsigned(cols), 1), s, p, grid);
         } else {
             launch_fold(attend_paged_fold_kernel<HD, NT, HD / 4, false>, dim3(unsigned(grid - 1), unsigned(cols), 1), s, p, grid);

@@ -7,8 +7,8 @@
 // symmetric rule the sixteenth never is).  The scale keeps eight bits because a code less 8 has at most three more:
 // their product is then EXACT in FP16, and attention can widen a cell to one FP16 operand instead of two (a rounded one
 // and its residual, as it needs for the 8-bit formats).  Against a scale of eleven bits this moves a value by at most
-// 2^-9 of itself, next to a quantisation step of 1/8 of the group's largest.  |d| stops at 2720 (values at 21760) because
-// the widening in attention multiplies by d and subtracts 24 d, and both have to be FP16 numbers.
+// 2^-9 of itself, next to a quantisation step of 1/8 of the group's largest.  |d| stops at 2720 (values at 21760), so that
+// a reader can widen in FP16 either way: subtract 8 first, as attention here does, or multiply first, as (code + 16) d - 24 d.
 // A group that holds an infinity or a NaN gets the scale NaN: the fault shows in whatever reads the cell.
 //
 // Planes are head-major, [kv_head][slot][head_dim / 2] bytes and [kv_head][slot][head_dim / 32] FP16 scales: a page of
