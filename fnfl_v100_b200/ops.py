@@ -421,8 +421,8 @@ def attend_paged_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      workspace: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q [rows][n_q][hd] over the paged KV4 cache: request r's rows are row_start[r] .. row_start[r + 1] - 1 (None:
     one row a request) and see its n_cells[r] cells, the pages table[r] lists, causally.  max_rows: the most rows of a request
-    (a hint).  Rows of no request are left as they were in `out`.  `workspace` (uint8) is used when it is large enough, else one
-    is allocated.  Returns out [rows][n_q][hd]."""
+    (a hint).  Rows of no request are left as they were in `out`, which may not overlap an input.  `workspace` (uint8) is used
+    when it is large enough, else one is allocated.  Returns out [rows][n_q][hd]."""
     _dev(q, torch.float32, "q")
     n_kv, slots, hd = _kv4_planes(k_cache, k_scale, "k")
     if q.dim() != 3 or q.shape[2] != hd or _kv4_planes(v_cache, v_scale, "v") != (n_kv, slots, hd):

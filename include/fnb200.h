@@ -456,17 +456,20 @@ int32_t fnb_attend_static(const fnb_attend_args * args, void * stream);
  * the device, so one captured graph serves every step; fnb_page_tables writes them.  A row that sees no cell gives
  * zeros; rows that belong to no request are left as they were.  What lies in a page behind a request's last cell, or in
  * cells a row does not see, does not touch its result, NaN included.
- * max_rows (a hint; 0 means 1): the most rows a request has.  Requests of at most max_rows rows have their cells read
- * once; up to 64 query rows a KV head (rows x n_q_heads / n_kv_heads) are served in one pass.
+ * max_rows (a hint; 0 means 1): the most rows a request has.  The query columns of a KV head (rows x n_q_heads /
+ * n_kv_heads) are served eight to a pass over its cells, sixteen when head_dim is 256 and max_rows gives more than eight;
+ * more columns are more passes, read mostly from L2.  A wrong hint costs time, not results.
  * F32 softmax statistics; products on the tensor cores with queries and probabilities split into two FP16 parts, cells
- * exact: relative error (2-norm) against a 64-bit evaluation about 1e-6.  |q| below 2^64.
+ * exact: relative error (2-norm) against a 64-bit evaluation about 5e-7.  |q| below 2^64.
  * A page id outside the cache, a length outside [0, max_pages page_size], or a row range outside [0, rows) sets
  * FNB_ERR_PAGES; the rows of that request then mean nothing, others are unaffected.
- * head_dim 64, 128 or 256; n_req in [1, 2048]; page_size a power of two from 16 on; cache_slots a multiple of page_size;
- * q, gate, out, caches and scales 16-byte aligned.  out may not overlap an input.
+ * head_dim 64, 128 or 256; n_req in [1, 2048]; page_size a power of two from 16 to 2^20; cache_slots a multiple of it
+ * below 2^31, cache_slots n_kv_heads below 2^32; n_q_heads a multiple of n_kv_heads up to 1024, rows n_q_heads below 2^31;
+ * q, gate, out, caches and scales 16-byte aligned.  out may not overlap an input.  The tiles to visit (128 cells, 256 when
+ * head_dim is below 256; times passes and KV heads, over all requests) number below 2^31: else FNB_ERR_PAGES, nothing written.
  * workspace: at least fnb_attend_paged_workspace_bytes(args) bytes (a function of head_dim, max_rows, the head counts
- * and whether max_pages page_size exceeds 128, not of the lengths), 16-byte aligned; its contents need no
- * initialisation and mean nothing afterwards.  Calls that share a workspace must not overlap on the GPU.
+ * and whether max_pages page_size exceeds 256, not of the lengths; up to 256 none is needed and null is taken), 16-byte
+ * aligned; its contents need no initialisation and mean nothing afterwards.  Calls that share a workspace must not overlap on the GPU.
  * The first call per device and shape class raises a kernel attribute (fnb_prepare_device covers it).
  * The reference attends one dense range per call (fn/kernels/qsa/attend.h:9-23); pages have no counterpart there.
  */

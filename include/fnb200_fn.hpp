@@ -22,6 +22,7 @@ namespace fnb {
 constexpr uint32_t err_token = FNB_ERR_TOKEN;      // fn::xchg::err_token's role
 constexpr uint32_t err_slot = FNB_ERR_SLOT;
 constexpr uint32_t err_timeout = FNB_ERR_TIMEOUT;
+constexpr uint32_t err_pages = FNB_ERR_PAGES;
 
 namespace draft {  // hidden RMSNorm: fn::draft::dcp_norm's arithmetic, F32 out
 
@@ -199,6 +200,36 @@ inline bool kv_read(const void * cache, const uint16_t * scale, const int32_t * 
     a.rows = rows, a.cache_slots = max_cells, a.cell0 = cell0, a.n_kv_heads = n_kv_heads, a.head_dim = head_dim;
     return fnb_kv_read_f32(&a, stream) == FNB_OK;
 }
+
+// ---- the paged KV4 cache: no counterpart in the reference, whose cache is one dense range per sequence
+
+// qsp_kv into head-major KV4 planes: k_cache / v_cache codes [n_kv_heads][max_cells][head_dim / 2], k_scale / v_scale FP16
+// [n_kv_heads][max_cells][head_dim / 32], all four required; a cell of -1 (page_tables' padding) is passed over
+inline bool qsp_kv4(const qsp_kv_args & a, void * stream) {
+    fnb_rope_kv8_args w{};
+    w.base.q = a.q, w.base.k = a.kv_k, w.base.v = a.kv_v, w.base.pos = a.pos, w.base.slots = a.cells;
+    w.base.q_norm_w = a.q_norm, w.base.k_norm_w = a.k_norm, w.base.q_out = a.q_out;
+    w.base.k_cache = a.k_cache, w.base.v_cache = a.v_cache, w.base.k_f32 = a.k_f32, w.base.err = a.err;
+    w.base.rows = a.rows, w.base.cache_slots = a.max_cells;
+    w.base.n_q_heads = a.n_q_heads, w.base.n_kv_heads = a.n_kv_heads, w.base.head_dim = a.head_dim;
+    w.base.n_rot = a.n_rot, w.base.theta_scale = a.theta_scale, w.base.eps = a.eps, w.base.planes = a.planes;
+    w.k_scale = a.k_scale, w.v_scale = a.v_scale;
+    return fnb_rope_neox_kv4_append(&w, stream) == FNB_OK;
+}
+// one KV4 plane's cells as F32 rows [rows][n_kv_heads][head_dim]; cells null: rows cell0 .. cell0 + rows - 1
+inline bool kv4_read(const void * cache, const uint16_t * scale, const int32_t * cells, int64_t cell0, int64_t rows,
+                     int64_t max_cells, int32_t n_kv_heads, int32_t head_dim, float * out, uint32_t * err, void * stream) {
+    fnb_kv_read_args a{};
+    a.cache = cache, a.scale = scale, a.cells = cells, a.out = out, a.err = err;
+    a.rows = rows, a.cache_slots = max_cells, a.cell0 = cell0, a.n_kv_heads = n_kv_heads, a.head_dim = head_dim;
+    return fnb_kv4_read_f32(&a, stream) == FNB_OK;
+}
+// block tables, slots and positions of a step; attention of all its requests over their pages
+using page_tables_args = fnb_page_tables_args;
+inline bool page_tables(const page_tables_args & a, void * stream) { return fnb_page_tables(&a, stream) == FNB_OK; }
+using attend_paged_args = fnb_attend_paged_args;
+inline size_t attend_paged_workspace(const attend_paged_args & a) { return fnb_attend_paged_workspace_bytes(&a); }
+inline bool attend_paged(const attend_paged_args & a, void * stream) { return fnb_attend_paged_kv4(&a, stream) == FNB_OK; }
 
 }  // namespace qsa
 
