@@ -39,7 +39,7 @@
 // scheduler.  The change took 61 us to 50 at 196 608 cells.)
 //
 // Measured on a B200, graph replays over caches larger than L2: one request of 196 608 cells, 16 heads over 2 of 256:
-// 43.2 us, 113 MB at 2.6 TB/s; 40 requests of up to 8192 cells, 32 heads over 8 of 128: 58 us; 8 requests of up to 300
+// 43.2 us, 113 MB at 2.6 TB/s; 40 requests of up to 5000 cells, 32 heads over 8 of 128: 51 us; 8 requests of up to 300
 // cells: 10.3 us, latency.  In its steady state a warp issues some 790 instructions a tile at 0.56 to 0.6 an issue slot,
 // the logic, FP16 and tensor units each 35 to 40 % busy; cells that lie in L2 give the same time.
 #include <atomic>
@@ -56,13 +56,17 @@ constexpr float kLog2eF = 1.4426950408889634f;
 constexpr float kPShift = 14.0f;                 // probabilities are held times 2^14
 
 // ---- geometry -------------------------------------------------------------------------------------------------------
-// HD: head_dim.  NT: blocks of eight query columns a unit serves (1, or 2 at 256).
-template <int HD, int NT>
+// HD: head_dim.  NT: blocks of eight query columns a unit serves (1, or 2 at 256); 0: four columns, whose large and small
+// parts fill one block (columns 0 .. 3 and 4 .. 7), so that one product does for both and the two halves of its result
+// are added at the end of the scores and of the item.
+template <int HD, int NT0>
 struct geo {
+    static constexpr bool kPacked = NT0 == 0;
+    static constexpr int NT = kPacked ? 1 : NT0, kParts = kPacked ? 1 : 2;   // words of a fragment: both parts, or either
     static constexpr int kGroups = HD / 32;                     // scales of a cell; also 32-dim groups of the output
     // cells of a tile: what a tile costs whatever its cells (the barrier, the walk, addresses) is the same for narrow heads
     static constexpr int kTile = NT == 1 && HD < 256 ? 256 : 128, kSets = kTile / 128, kSlabs = kTile / 16;
-    static constexpr int kCols = 8 * NT;
+    static constexpr int kCols = kPacked ? 4 : 8 * NT;
     static constexpr int kWarps = 8, kThreads = kWarps * 32;
     static constexpr int kCellGroups = 8 / kGroups;             // warps that share a dim group (and columns) split the cells
     static constexpr int kCodeBytes = kTile * HD / 2, kScaleBytes = kTile * kGroups * 2;
@@ -73,16 +77,17 @@ struct geo {
     static constexpr uint32_t kSwz = HD == 256 ? 7u : HD == 128 ? 3u : 1u;
     // shared memory
     static constexpr int ring = 0;
-    static constexpr int prob = ring + kStages * kUnitBytes;    // uint4 [2][kSlabs][NT][32]
-    static constexpr int qfrag = prob + 2 * kSlabs * NT * 512;       // uint4 [NT][kGroups][hi, lo][32]
-    static constexpr int wmax = qfrag + NT * kGroups * 1024;    // float [2][kWarps][kCols]; and the queries' [kGroups][kCols]
+    static constexpr int prob = ring + kStages * kUnitBytes;    // uint4 (uint2) [2][kSlabs][NT][32]
+    static constexpr int qfrag = prob + 2 * kSlabs * NT * kParts * 256;   // uint4 [NT][kGroups][kParts][32]
+    static constexpr int kQueryBytes = NT * kGroups * kParts * 512;
+    static constexpr int wmax = qfrag + kQueryBytes;    // float [2][kWarps][kCols]; and the queries' [kGroups][kCols]
     static constexpr int lsum = wmax + 2 * 8 * kCols * 4;       // float [kWarps][kCols]
     static constexpr int corr = lsum + 8 * kCols * 4;           // float [2][kCols]
     static constexpr int mfin = corr + 2 * kCols * 4;           // float [kCols]
     // float4: the other cell groups' accumulators.  Of 128-wide heads they fit where the queries were: those are read up to
     // the item's last scores, and the next item's are written behind a barrier of its own.
-    static constexpr int kRedBytes = (kCellGroups - 1) * kGroups * 32 * kCols * 4, tail = mfin + kCols * 4;
-    static constexpr bool kRedOnQueries = kRedBytes <= NT * kGroups * 1024;
+    static constexpr int kRedBytes = (kCellGroups - 1) * kGroups * NT * 1024, tail = mfin + kCols * 4;
+    static constexpr bool kRedOnQueries = kRedBytes <= kQueryBytes;
     static constexpr int red = kRedOnQueries ? qfrag : tail;
     static constexpr int scan = tail + (kRedOnQueries ? 0 : kRedBytes);  // int64 [kWarps]: sums; the piece's start
     static constexpr int total = scan + (kWarps + 4) * 8 + 1024;          // + slack to align the base to 1024 bytes
@@ -251,9 +256,8 @@ struct __align__(16) fold_head {
 // id a warp and tile, fetched a step ahead, and addresses that differ by constants.  A lane copies one 16-byte chunk (a
 // group's codes) of kPass rows, and one row's scales, K's (lower half-warp) or V's.  Chunk c of a row lies at c ^ (bits
 // of the row), which keeps ldmatrix free of bank conflicts.  The walk runs two tiles ahead of the scores.
-template <int HD, int NT>
+template <class G, int HD>
 struct loader {
-    using G = geo<HD, NT>;
     static constexpr int kCh = G::kGroups, kRows = 32 / kCh, kPass = 16 / kRows, kRow = HD / 2, kScale = kCh * 2;
     static constexpr int kLag = 4 - G::kVStages, S = G::kSets;  // a tile is S sets of 128 rows, sixteen to a warp
     cursor<G> c;
@@ -362,11 +366,12 @@ struct loader {
 };
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------
-template <int HD, int NT>
-__global__ void __launch_bounds__(geo<HD, NT>::kThreads, geo<HD, NT>::kCtas)
+template <int HD, int NT0>
+__global__ void __launch_bounds__(geo<HD, NT0>::kThreads, geo<HD, NT0>::kCtas)
 attend_paged_kernel(const __grid_constant__ paged_params p) {
-    using G = geo<HD, NT>;
-    constexpr int NB = G::kGroups;
+    using G = geo<HD, NT0>;
+    constexpr int NB = G::kGroups, NT = G::NT, kParts = G::kParts;
+    constexpr bool kPacked = G::kPacked;
     extern __shared__ uint8_t smem_raw[];
     uint8_t * smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (rounding the pointer itself would make every access a generic one)
     int64_t * s_scan = reinterpret_cast<int64_t *>(smem + G::scan);
@@ -440,7 +445,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     c.at(p, int(s_start[0]), s_start[1]);
     if (p.whole) c.tile = 0;
     const uint32_t ring = smem_u32(smem) + G::ring;
-    loader<HD, NT> load;
+    loader<G, HD> load;
     load.start(p, c, u1 - u0, ring);
     if (tid == G::kThreads - 1 && p.ws_head != nullptr) {
         fold_head f = {0, 0, 0, c.h, c.blk, c.x.row0, c.x.m, 0};
@@ -453,6 +458,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     }
 
     const int g = lane >> 2, t = lane & 3;
+    const int t2 = kPacked ? 2 * (t & 1) : 2 * t;                    // of a block's columns, this lane's first in a product's result
     constexpr int SL = G::kSets;                                     // scores: a warp's slabs of 16 cells, wid SL on
     const int dg = wid % NB, cg = wid / NB;                          // outputs: dim group, cell group
     constexpr int kSlabs = G::kSlabs / G::kCellGroups;                       // slabs of a cell group
@@ -460,7 +466,8 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     float * s_lsum = reinterpret_cast<float *>(smem + G::lsum);
     float * s_corr = reinterpret_cast<float *>(smem + G::corr);
     float * s_mfin = reinterpret_cast<float *>(smem + G::mfin);
-    uint4 * s_prob = reinterpret_cast<uint4 *>(smem + G::prob);
+    using frag = std::conditional_t<kPacked, uint2, uint4>;          // probabilities of a slab, a lane's
+    frag * s_prob = reinterpret_cast<frag *>(smem + G::prob);
     uint4 * s_q = reinterpret_cast<uint4 *>(smem + G::qfrag);
     // ldmatrix: a lane's row of a tile and its 16-byte chunk there, which the loader has xored with bits of the row
     // (the same for every sixteenth row, so all addresses of a lane differ by constants)
@@ -483,7 +490,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         // of column 8 x + g, which are nibbles 0 .. 3 of the two halves of a cell's word.  A (column block, group) at a time
         // a warp; the rows' maxima and then the fragments cross the warps.
         auto load8 = [&](int b, int x, float4 (&v)[2]) {
-            const int col = x * 8 + g, i = row_of_col(col);
+            const int col = kPacked ? g & 3 : x * 8 + g, i = row_of_col(col);
             const float * src = p.q + (int64_t(c.x.row0 + i) * p.n_q + c.h * p.group + (col0 + col - i * p.group)) * HD + 32 * b + 8 * t;
             const bool on = i < c.x.m;
             v[0] = on ? __ldg(reinterpret_cast<const float4 *>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -514,7 +521,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                               fmaxf(fmaxf(fabsf(v[1].x), fabsf(v[1].y)), fmaxf(fabsf(v[1].z), fabsf(v[1].w))));
             top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
             top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-            if (t == 0) s_wmax[b * G::kCols + x * 8 + g] = top;
+            if (t == 0) s_wmax[b * G::kCols + (kPacked ? g & 3 : x * 8 + g)] = top;
         }
         if (load.step == 1) load.next(p, ring);
         named_barrier<1>(G::kThreads);
@@ -525,22 +532,26 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             float4 v[2] = {first[0], first[1]};
             if (k > 0) load8(b, x, v);                       // again, from L1
             float up, down;
-            powers(top_of(x * 8 + g), up, down);
+            powers(top_of(kPacked ? g & 3 : x * 8 + g), up, down);
             uint4 hi, lo;
             split2(__fmul_rn(v[0].x, up), __fmul_rn(v[1].x, up), hi.x, lo.x);
             split2(__fmul_rn(v[0].y, up), __fmul_rn(v[1].y, up), hi.y, lo.y);
             split2(__fmul_rn(v[0].z, up), __fmul_rn(v[1].z, up), hi.z, lo.z);
             split2(__fmul_rn(v[0].w, up), __fmul_rn(v[1].w, up), hi.w, lo.w);
-            s_q[(x * NB + b) * 64 + lane] = hi, s_q[(x * NB + b) * 64 + 32 + lane] = lo;
+            if constexpr (kPacked) {
+                s_q[b * 32 + lane] = g < 4 ? hi : lo;
+            } else {
+                s_q[(x * NB + b) * 64 + lane] = hi, s_q[(x * NB + b) * 64 + 32 + lane] = lo;
+            }
         }
-        // columns 8 x + 2 t + z: the factor of their scores, the cells they see; running maxima, this warp's sums
+        // columns 8 x + t2 + z: the factor of their scores, the cells they see; running maxima, this warp's sums
         float sc[NT][2], mx[NT][2], ls[NT][2];
         int lim[NT][2];
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
-                const int col = x * 8 + 2 * t + z, r = row_of_col(col);
+                const int col = x * 8 + t2 + z, r = row_of_col(col);
                 float up, down;
                 powers(top_of(col), up, down);
                 sc[x][z] = fmaxf(p.scale_log2 * down, 0x1p-126f);
@@ -607,17 +618,24 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                     if (NT > 1 && x >= n_blocks) break;
                     uint4 hi[2], lo[2];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) hi[j] = s_q[(x * NB + b + j) * 64 + lane], lo[j] = s_q[(x * NB + b + j) * 64 + 32 + lane];
+                    for (int j = 0; j < 2; ++j) hi[j] = s_q[(x * NB + b + j) * kParts * 32 + lane];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) if (!kPacked) lo[j] = s_q[(x * NB + b + j) * 64 + 32 + lane];
 #pragma unroll
                     for (int s = 0; s < SL; ++s) {
                         // two groups side by side, so that their sums' chains overlap; the small parts first
                         float part[2][4];
+                        if constexpr (kPacked) {
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) mma16816_first(part[j], ka[s][j][0], ka[s][j][1], ka[s][j][2], ka[s][j][3], lo[j].x, lo[j].y);
+                            for (int j = 0; j < 2; ++j) mma16816_first(part[j], ka[s][j][0], ka[s][j][1], ka[s][j][2], ka[s][j][3], hi[j].x, hi[j].y);
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) mma16816(part[j], ka[s][j][4], ka[s][j][5], ka[s][j][6], ka[s][j][7], lo[j].z, lo[j].w);
+                            for (int j = 0; j < 2; ++j) mma16816_first(part[j], ka[s][j][0], ka[s][j][1], ka[s][j][2], ka[s][j][3], lo[j].x, lo[j].y);
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) mma16816(part[j], ka[s][j][0], ka[s][j][1], ka[s][j][2], ka[s][j][3], hi[j].x, hi[j].y);
+                            for (int j = 0; j < 2; ++j) mma16816(part[j], ka[s][j][4], ka[s][j][5], ka[s][j][6], ka[s][j][7], lo[j].z, lo[j].w);
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) mma16816(part[j], ka[s][j][0], ka[s][j][1], ka[s][j][2], ka[s][j][3], hi[j].x, hi[j].y);
+                        }
 #pragma unroll
                         for (int j = 0; j < 2; ++j) mma16816(part[j], ka[s][j][4], ka[s][j][5], ka[s][j][6], ka[s][j][7], hi[j].z, hi[j].w);
                         const float2 f0 = __half22float2(u32_h2(dk[s][0][b / 2])), f1 = __half22float2(u32_h2(dk[s][1][b / 2]));
@@ -628,6 +646,13 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                             sv[s][x][2] = fmaf(c, part[j][2], sv[s][x][2]), sv[s][x][3] = fmaf(c, part[j][3], sv[s][x][3]);
                         }
                     }
+                }
+            }
+            if constexpr (kPacked) {  // the large parts' sums and the small parts'
+#pragma unroll
+                for (int s = 0; s < SL; ++s) {
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) sv[s][0][z] += __shfl_xor_sync(kFull, sv[s][0][z], 2);
                 }
             }
             if (base + G::kTile > lim_min) {
@@ -651,7 +676,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                 for (int s = 0; s < SL; ++s) t0 = fmaxf(t0, fmaxf(sv[s][x][0], sv[s][x][2])), t1 = fmaxf(t1, fmaxf(sv[s][x][1], sv[s][x][3]));
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) t0 = fmaxf(t0, __shfl_xor_sync(kFull, t0, o)), t1 = fmaxf(t1, __shfl_xor_sync(kFull, t1, o));
-                if (g == 0) *reinterpret_cast<float2 *>(s_wmax + ((it & 1) * 8 + wid) * G::kCols + x * 8 + 2 * t) = make_float2(t0, t1);
+                if (g == 0) *reinterpret_cast<float2 *>(s_wmax + ((it & 1) * 8 + wid) * G::kCols + x * 8 + t2) = make_float2(t0, t1);
             }
         };
         // probabilities of tile `it`, in the second product's fragment order; the factor its outputs rescale the sums by
@@ -660,7 +685,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             for (int x = 0; x < NT; ++x) {
                 if (NT > 1 && x >= n_blocks) break;
                 // lane (g, t) takes the maxima that the g-th warp found
-                float2 v = *reinterpret_cast<const float2 *>(s_wmax + ((it & 1) * 8 + g) * G::kCols + x * 8 + 2 * t);
+                float2 v = *reinterpret_cast<const float2 *>(s_wmax + ((it & 1) * 8 + g) * G::kCols + x * 8 + t2);
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) v.x = fmaxf(v.x, __shfl_xor_sync(kFull, v.x, o)), v.y = fmaxf(v.y, __shfl_xor_sync(kFull, v.y, o));
                 const float n0 = fmaxf(mx[x][0], v.x * sc[x][0]), n1 = fmaxf(mx[x][1], v.y * sc[x][1]);
@@ -678,8 +703,12 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                     uint32_t h0, h1, q0, q1;
                     split2(e0, e1, h0, q0);
                     split2(e2, e3, h1, q1);
-                    s_prob[(((it & 1) * G::kSlabs + wid * SL + s) * NT + x) * 32 + lane] =
-                        make_uint4(transpose8x8(h0), transpose8x8(h1), transpose8x8(q0), transpose8x8(q1));
+                    frag & to = s_prob[(((it & 1) * G::kSlabs + wid * SL + s) * NT + x) * 32 + lane];
+                    if constexpr (kPacked) {
+                        to = make_uint2(transpose8x8(t < 2 ? h0 : q0), transpose8x8(t < 2 ? h1 : q1));
+                    } else {
+                        to = make_uint4(transpose8x8(h0), transpose8x8(h1), transpose8x8(q0), transpose8x8(q1));
+                    }
                 }
             }
         };
@@ -702,7 +731,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                     if ((dv[(lane + 32 * j) * NB] & 0x7c00u) == 0x7c00u) bad |= 1u << j;
                 }
             }
-            // the tile's sums: with one column block the small parts apart, which halves the chains
+            // the tile's sums: with one column block the small parts (of four columns every second slab) apart: shorter chains
             float part[NT][2][4], small[2][4];
 #pragma unroll
             for (int z = 0; z < 4; ++z) {
@@ -736,16 +765,18 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
 #pragma unroll
                     for (int x = 0; x < NT; ++x) {
                         if (NT > 1 && x >= n_blocks) break;
-                        const uint4 f = s_prob[(((it & 1) * G::kSlabs + cg * kSlabs + sp + j) * NT + x) * 32 + lane];
-                        if constexpr (NT == 1) {
-                            mma16816(small[0], a0, a1, a2, a3, f.z, f.w);
-                            mma16816(small[1], b0, b1, b2, b3, f.z, f.w);
+                        const frag f = s_prob[(((it & 1) * G::kSlabs + cg * kSlabs + sp + j) * NT + x) * 32 + lane];
+                        if constexpr (kPacked) {
+                            mma16816(j ? small[0] : part[0][0], a0, a1, a2, a3, f.x, f.y);
+                            mma16816(j ? small[1] : part[0][1], b0, b1, b2, b3, f.x, f.y);
                         } else {
-                            mma16816(part[x][0], a0, a1, a2, a3, f.z, f.w);
-                            mma16816(part[x][1], b0, b1, b2, b3, f.z, f.w);
+                            float(&s0)[4] = NT == 1 ? small[0] : part[x][0];
+                            float(&s1)[4] = NT == 1 ? small[1] : part[x][1];
+                            mma16816(s0, a0, a1, a2, a3, f.z, f.w);
+                            mma16816(s1, b0, b1, b2, b3, f.z, f.w);
+                            mma16816(part[x][0], a0, a1, a2, a3, f.x, f.y);
+                            mma16816(part[x][1], b0, b1, b2, b3, f.x, f.y);
                         }
-                        mma16816(part[x][0], a0, a1, a2, a3, f.x, f.y);
-                        mma16816(part[x][1], b0, b1, b2, b3, f.x, f.y);
                     }
                 }
             }
@@ -770,7 +801,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                     for (int x = 0; x < NT; ++x) {
 #pragma unroll
                         for (int z = 0; z < 2; ++z) {
-                            if (base + cg * kSlabs * 16 + cell >= c.x.n - c.x.m + row_of_col(x * 8 + 2 * t + z) + 1) continue;
+                            if (base + cg * kSlabs * 16 + cell >= c.x.n - c.x.m + row_of_col(x * 8 + t2 + z) + 1) continue;
 #pragma unroll
                             for (int y = 0; y < 2; ++y) acc[x][y][z] = acc[x][y][z + 2] = NAN;
                         }
@@ -813,8 +844,15 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                 ls[x][0] += __shfl_xor_sync(kFull, ls[x][0], o), ls[x][1] += __shfl_xor_sync(kFull, ls[x][1], o);
             }
             if (g == 0) {
-                *reinterpret_cast<float2 *>(s_lsum + wid * G::kCols + x * 8 + 2 * t) = make_float2(ls[x][0], ls[x][1]);
-                if (wid == 0) *reinterpret_cast<float2 *>(s_mfin + x * 8 + 2 * t) = make_float2(mx[x][0], mx[x][1]);
+                *reinterpret_cast<float2 *>(s_lsum + wid * G::kCols + x * 8 + t2) = make_float2(ls[x][0], ls[x][1]);
+                if (wid == 0) *reinterpret_cast<float2 *>(s_mfin + x * 8 + t2) = make_float2(mx[x][0], mx[x][1]);
+            }
+        }
+        if constexpr (kPacked) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+#pragma unroll
+                for (int z = 0; z < 4; ++z) acc[0][y][z] += __shfl_xor_sync(kFull, acc[0][y][z], 2);
             }
         }
         float4 * s_red = reinterpret_cast<float4 *>(smem + G::red);
@@ -845,8 +883,8 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             for (int x = 0; x < NT; ++x) {
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
-                    if (NT > 1 && x >= n_blocks) continue;
-                    const int col = x * 8 + 2 * t + z, i = row_of_col(col);
+                    if ((NT > 1 && x >= n_blocks) || (kPacked && t >= 2)) continue;
+                    const int col = x * 8 + t2 + z, i = row_of_col(col);
                     if (i >= c.x.m) continue;
                     float l = 0.0f;
 #pragma unroll
@@ -881,9 +919,9 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
 // idle).  Else block k looks at piece k + 1 alone, which costs one load where there is nothing to fold.
 constexpr int kFoldThreads = 256;
 constexpr int kMaxPieces = 2 * kSmCount;
-template <int HD, int NT, int VEC, bool LISTED>
+template <int HD, int COLS, int VEC, bool LISTED>
 __global__ void __launch_bounds__(kFoldThreads) attend_paged_fold_kernel(const __grid_constant__ paged_params p, const int pieces_all) {
-    constexpr int COLS = 8 * NT, SPLIT = kFoldThreads / VEC;
+    constexpr int SPLIT = kFoldThreads / VEC;
     __shared__ float4 s_acc[SPLIT][VEC];
     __shared__ float s_max[kFoldThreads / 32], s_sum[kFoldThreads / 32];
     __shared__ float s_weight[kMaxPieces], s_part[kMaxPieces];
@@ -1006,13 +1044,17 @@ bool configure() {
     return true;
 }
 
-// Column blocks of eight a unit serves.  A 256-wide head's cells are read once for sixteen columns where a request has
+// Column blocks of eight a unit serves, or 0.  A 256-wide head's cells are read once for sixteen columns where a request has
 // that many; further columns are further passes.  (196 608 cells of 2 heads: two rows, 16 columns a head, 66 us against 75
 // in two passes; eight rows, 64 columns, 215 us against 231 and 270 with units of 32 and 64 columns, whose sums leave
 // registers for one CTA an SM.)  Narrow heads fare better with one block and the larger tiles it leaves room for (32
-// requests of up to 4096 cells, 8 heads of 128, eight rows of four: 92 us against 97).
+// requests of up to 4096 cells, 8 heads of 128, eight rows of four: 92 us against 97).  Up to four columns share a block
+// between their large and small parts, 0 here: half the products (40 requests of up to 5000 cells, 32 heads over 8 of 128:
+// 51 us against 58; 196 608 cells, 8 over 2 of 256: 36.8 against 42.7).  64-wide heads, whose tiles hold the least work next
+// to what a tile costs anyway, have nothing from it (32 requests, 32 over 8: 35.5 against 33.9).
 int column_blocks(const fnb_attend_paged_args * a) {
     const int64_t cols = int64_t(a->max_rows > 0 ? a->max_rows : 1) * (a->n_q_heads / a->n_kv_heads);
+    if (cols <= 4 && a->head_dim >= 128) return 0;
     return a->head_dim == 256 && cols > 8 ? 2 : 1;
 }
 constexpr int kGrid = 2 * kSmCount;  // two CTAs an SM
@@ -1024,7 +1066,7 @@ bool whole_items(const fnb_attend_paged_args * a) { return int64_t(a->max_pages)
 size_t paged_workspace(const fnb_attend_paged_args * a) {
     if (whole_items(a)) return 16;  // none is used
     const int nt = column_blocks(a);
-    const size_t grid = size_t(kGrid), cols = size_t(8 * nt);
+    const size_t grid = size_t(kGrid), cols = nt == 0 ? 4 : size_t(8 * nt);
     return grid * 2 * cols * (size_t(a->head_dim) + 2) * 4 + grid * 32;
 }
 
@@ -1055,7 +1097,8 @@ template <int HD, int NT>
 int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStream_t s) {
     if (!configure<HD, NT>()) return FNB_LAUNCH_FAILED;
     const int grid = kGrid;
-    const size_t cols = 8 * NT;
+    constexpr int kCols = geo<HD, NT>::kCols;
+    const size_t cols = kCols;
     const bool fold = !p.whole;
     if (fold) {
         uint8_t * ws = static_cast<uint8_t *>(a->workspace);
@@ -1071,18 +1114,21 @@ int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStre
         const int64_t items = int64_t(a->n_req) * a->n_kv_heads * blocks;
         const int64_t outputs = items * int64_t(cols), wave = kSmCount * 8;   // columns to fold; blocks that run at a time
         if (outputs * (HD / 32) <= wave && p.cells_max >= 64 * 128) {
-            launch_fold(attend_paged_fold_kernel<HD, NT, 8, true>, dim3(unsigned(items), unsigned(cols), HD / 32), s, p, grid);
+            launch_fold(attend_paged_fold_kernel<HD, kCols, 8, true>, dim3(unsigned(items), unsigned(cols), HD / 32), s, p, grid);
         } else if (outputs <= wave) {
-            launch_fold(attend_paged_fold_kernel<HD, NT, HD / 4, true>, dim3(unsigned(items), unsigned(cols), 1), s, p, grid);
+            launch_fold(attend_paged_fold_kernel<HD, kCols, HD / 4, true>, dim3(unsigned(items), unsigned(cols), 1), s, p, grid);
         } else {
-            launch_fold(attend_paged_fold_kernel<HD, NT, HD / 4, false>, dim3(unsigned(grid - 1), unsigned(cols), 1), s, p, grid);
+            launch_fold(attend_paged_fold_kernel<HD, kCols, HD / 4, false>, dim3(unsigned(grid - 1), unsigned(cols), 1), s, p, grid);
         }
     }
     return launch_status();
 }
 }  // namespace
 
-bool attend_paged_prepare_device() { return configure<256, 1>() && configure<256, 2>() && configure<128, 1>() && configure<64, 1>(); }
+bool attend_paged_prepare_device() {
+    return configure<256, 0>() && configure<256, 1>() && configure<256, 2>() && configure<128, 0>() && configure<128, 1>() &&
+           configure<64, 1>();
+}
 
 }  // namespace fnb
 
@@ -1116,6 +1162,10 @@ extern "C" int32_t fnb_attend_paged_kv4(const fnb_attend_paged_args * a, void * 
     p.whole = whole_items(a);
     p.e1024 = 0x64006400u, p.e64 = 0x54005400u;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a->head_dim == 256) return column_blocks(a) == 2 ? launch_paged<256, 2>(a, p, s) : launch_paged<256, 1>(a, p, s);
-    return a->head_dim == 128 ? launch_paged<128, 1>(a, p, s) : launch_paged<64, 1>(a, p, s);
+    const int blocks = column_blocks(a);
+    switch (a->head_dim) {
+        case 256: return blocks == 0 ? launch_paged<256, 0>(a, p, s) : blocks == 1 ? launch_paged<256, 1>(a, p, s) : launch_paged<256, 2>(a, p, s);
+        case 128: return blocks == 0 ? launch_paged<128, 0>(a, p, s) : launch_paged<128, 1>(a, p, s);
+        default: return launch_paged<64, 1>(a, p, s);
+    }
 }

@@ -457,8 +457,8 @@ int32_t fnb_attend_static(const fnb_attend_args * args, void * stream);
  * zeros; rows that belong to no request are left as they were.  What lies in a page behind a request's last cell, or in
  * cells a row does not see, does not touch its result, NaN included.
  * max_rows (a hint; 0 means 1): the most rows a request has.  The query columns of a KV head (rows x n_q_heads /
- * n_kv_heads) are served eight to a pass over its cells, sixteen when head_dim is 256 and max_rows gives more than eight;
- * more columns are more passes, read mostly from L2.  A wrong hint costs time, not results.
+ * n_kv_heads) are served eight to a pass over its cells (four when max_rows gives no more and head_dim is at least 128,
+ * sixteen when it gives more than eight and head_dim is 256); more columns are more passes, read mostly from L2.  A wrong hint costs time, not results.
  * F32 softmax statistics; products on the tensor cores with queries and probabilities split into two FP16 parts, cells
  * exact: relative error (2-norm) against a 64-bit evaluation about 5e-7.  |q| below 2^64.
  * A page id outside the cache, a length outside [0, max_pages page_size], or a row range outside [0, rows) sets
