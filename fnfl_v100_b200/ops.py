@@ -404,7 +404,7 @@ def kv4_read_f32(cache: torch.Tensor, scale: torch.Tensor, *, cells: torch.Tenso
         rows = slots - cell0
     with _on(cache, scale, cells, out, _err(err)):
         if out is None:
-            out = torch.empty((rows, n_kv, hd), dtype=torch.float32, device=cache.device)
+            out = cache.new_empty((rows, n_kv, hd), dtype=torch.float32)
         else:
             _numel(_dev(out, torch.float32, "out"), rows * n_kv * hd, "out")
         a = _lib.KvReadArgs(cache.data_ptr(), scale.data_ptr(), _at(cells), out.data_ptr(), _at(err), rows, slots, cell0, n_kv, hd)
@@ -452,8 +452,8 @@ def attend_paged_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
             _dev(workspace, torch.uint8, "workspace")
         if need > _NO_WORKSPACE:
             if workspace is None or workspace.numel() < need:
-                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+                workspace = table.new_empty(-(-need // 4))
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), need
         _check(_lib.lib().fnb_attend_paged_kv4(C.byref(a), _raw_stream(q)), "attend_paged_kv4")
     return out
 
