@@ -27,7 +27,9 @@
 // requests form one line that is cut into equal pieces, one for each resident CTA, wherever the requests' borders fall:
 // one long request and many ragged ones both fill the machine, from lengths only the device knows.  A piece that holds
 // all tiles of an item writes its rows itself; otherwise it leaves its sums, maximum and accumulators in the workspace
-// and a second launch folds an item's pieces in their order.  Results do not depend on timing.
+// and a second launch folds an item's pieces in their order.  Where a table lists few cells and there are few items, an
+// item's tiles go to a cluster of CTAs instead, which join their parts through shared memory (share_of).  Results do not
+// depend on timing.
 //
 // A CTA is eight warps.  Scores: a warp takes 16 cells (32) for eight columns.  Maxima cross the warps through shared memory,
 // probabilities go there in the order of the second product's fragments, and there a warp takes 32 dims of all cells.
@@ -40,7 +42,7 @@
 //
 // Measured on a B200, graph replays over caches larger than L2: one request of 196 608 cells, 16 heads over 2 of 256:
 // 43.2 us, 113 MB at 2.6 TB/s; 40 requests of up to 5000 cells, 32 heads over 8 of 128: 51 us; 8 requests of up to 300
-// cells: 10.3 us, latency.  In its steady state a warp issues some 790 instructions a tile at 0.56 to 0.6 an issue slot,
+// cells: 8.1 us, latency.  In its steady state a warp issues some 790 instructions a tile at 0.56 to 0.6 an issue slot,
 // the logic, FP16 and tensor units each 35 to 40 % busy; cells that lie in L2 give the same time.
 #include <atomic>
 #include <type_traits>
@@ -53,6 +55,7 @@ namespace {
 
 constexpr int kMaxReq = 2048;
 constexpr float kLog2eF = 1.4426950408889634f;
+constexpr int kMaxShare = 8;                     // CTAs that share an item in the clustered form, at most
 constexpr float kPShift = 14.0f;                 // probabilities are held times 2^14
 
 // ---- geometry -------------------------------------------------------------------------------------------------------
@@ -112,6 +115,7 @@ struct paged_params {
     // at most group / 2^(31 + l) of 1 / group, so the product by less than 1 / group
     uint32_t group_mul, group_shift;
     bool whole;           // pieces begin where items do
+    int share_shift;      // log2 of the CTAs that share an item
 };
 
 // ---- small pieces -----------------------------------------------------------------------------------------------------
@@ -182,6 +186,26 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int LEFT>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
+// clusters: all threads of all CTAs arrive and wait; this address in another CTA's shared memory; loads from there
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t smem_of(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
 // A request as every thread that walks the units sees it.
 struct request {
     int n, m, row0;      // cells, rows, first row
@@ -204,8 +228,9 @@ __device__ __forceinline__ request load_request(const paged_params & p, int r, b
     x.blocks = int((int64_t(x.m) * p.group + G::kCols - 1) / G::kCols);
     return x;
 }
-__device__ __forceinline__ int64_t units_of(const paged_params & p, const request & x) {
-    return int64_t(p.n_kv) * x.blocks * x.tiles;
+template <bool ITEMS>
+__device__ __forceinline__ int64_t units_of(const paged_params & p, const request & x) {  // or its items
+    return int64_t(p.n_kv) * x.blocks * (ITEMS ? 1 : x.tiles);
 }
 
 // the walk over a piece of the line: request, KV head, column block, tile
@@ -220,6 +245,15 @@ struct cursor {
         tile = int(offset - item * uint32_t(x.tiles));
         h = int(item / uint32_t(x.blocks));
         blk = int(item - uint32_t(h) * uint32_t(x.blocks));
+    }
+    // CTA `rank` of those that share an item, the request's item-th: where its tiles begin, and their number
+    __device__ __forceinline__ int at_share(const paged_params & p, int request_index, uint32_t item, int rank) {
+        r = request_index;
+        x = load_request<G>(p, r, false);
+        h = int(item / uint32_t(x.blocks));
+        blk = int(item - uint32_t(h) * uint32_t(x.blocks));
+        tile = int(int64_t(x.tiles) * rank >> p.share_shift);
+        return int(int64_t(x.tiles) * (rank + 1) >> p.share_shift) - tile;
     }
     __device__ __forceinline__ void next_item(const paged_params & p) {
         tile = 0;
@@ -366,7 +400,9 @@ struct loader {
 };
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------
-template <int HD, int NT0>
+// SHARED: clusters of two to eight CTAs, each cluster an item at a time and each CTA an even share of its tiles; shares are
+// joined through the CTAs' shared memory, in the order of the tiles, and there is no second launch.
+template <int HD, int NT0, bool SHARED>
 __global__ void __launch_bounds__(geo<HD, NT0>::kThreads, geo<HD, NT0>::kCtas)
 attend_paged_kernel(const __grid_constant__ paged_params p) {
     using G = geo<HD, NT0>;
@@ -386,7 +422,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     int64_t mine = 0;
     for (int j = 0; j < per; ++j) {
         const int r = tid * per + j;
-        if (r < p.n_req) mine += units_of(p, load_request<G>(p, r, blockIdx.x == 0));
+        if (r < p.n_req) mine += units_of<SHARED>(p, load_request<G>(p, r, blockIdx.x == 0));
     }
     int64_t upto = mine;
 #pragma unroll
@@ -413,7 +449,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         if (u < total && upto > int64_t(u) && upto - mine <= int64_t(u)) {
             int64_t base = upto - mine;
             for (int j = 0; j < per; ++j) {
-                const int64_t units = units_of(p, load_request<G>(p, tid * per + j, false));
+                const int64_t units = units_of<SHARED>(p, load_request<G>(p, tid * per + j, false));
                 if (base + units > int64_t(u)) {
                     s_start[slot] = uint32_t(tid * per + j);
                     s_start[slot + 1] = u - uint32_t(base);
@@ -423,10 +459,17 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             }
         }
     };
+    [[maybe_unused]] const int rank = int(blockIdx.x) & ((1 << p.share_shift) - 1);   // in its cluster
+    [[maybe_unused]] uint32_t shared_item = blockIdx.x >> p.share_shift;
+    if constexpr (SHARED) u0 = shared_item;
     find(u0, 0);
-    if (p.whole) find(u1, 2);
+    if (!SHARED && p.whole) find(u1, 2);
     __syncthreads();
-    if (p.whole && u0 < u1) {
+    if constexpr (SHARED) {
+        if (shared_item >= total) return;   // the whole cluster
+        u0 = 0, u1 = 1;
+    }
+    if (!SHARED && p.whole && u0 < u1) {
         cursor<G> at;
         at.at(p, int(s_start[0]), s_start[1]);
         u0 -= uint32_t(at.tile);
@@ -442,12 +485,16 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         return;
     }
     cursor<G> c;
-    c.at(p, int(s_start[0]), s_start[1]);
-    if (p.whole) c.tile = 0;
+    if constexpr (SHARED) {
+        u1 = uint32_t(c.at_share(p, int(s_start[0]), s_start[1], rank));
+    } else {
+        c.at(p, int(s_start[0]), s_start[1]);
+        if (p.whole) c.tile = 0;
+    }
     const uint32_t ring = smem_u32(smem) + G::ring;
     loader<G, HD> load;
     load.start(p, c, u1 - u0, ring);
-    if (tid == G::kThreads - 1 && p.ws_head != nullptr) {
+    if (!SHARED && tid == G::kThreads - 1 && p.ws_head != nullptr) {
         fold_head f = {0, 0, 0, c.h, c.blk, c.x.row0, c.x.m, 0};
         if (c.tile != 0) {
             const uint32_t first = u0 - uint32_t(c.tile);          // the item's first unit
@@ -478,10 +525,10 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
 
     uint32_t k_at = G::ring, v_at = G::ring + 2 * G::kUnitBytes;  // stages of the next tile scored, of the next tile put out
     uint32_t u = u0;
-    while (u < u1) {
+    while (SHARED || u < u1) {
         const int tile_first = c.tile;
         const int n_tiles = int(min(uint32_t(c.x.tiles - c.tile), u1 - u));
-        const bool whole = tile_first == 0 && n_tiles == c.x.tiles;
+        const bool whole = tile_first == 0 && n_tiles == c.x.tiles;      // (a share may have no tiles)
         const int col0 = c.blk * G::kCols;
         auto row_of_col = [&](int col) { return int(uint64_t(uint32_t(col0 + col)) * p.group_mul >> p.group_shift); };  // / p.group
 
@@ -820,7 +867,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
 
         // One barrier a tile: behind it lie the tile's scores, the probabilities of the tile before and all copies begun
         // before the last barrier.  Between two barriers a warp has three pieces of work that do not wait for one another.
-        scores(0);
+        if (!SHARED || n_tiles > 0) scores(0);
         float r0 = 0.0f, r1 = 0.0f;
         for (int it = 0; it < n_tiles; ++it) {
             copies_wait<0>();
@@ -834,7 +881,7 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         }
         copies_wait<0>();
         named_barrier<1>(G::kThreads);
-        outputs(n_tiles - 1, r0, r1);
+        if (!SHARED || n_tiles > 0) outputs(n_tiles - 1, r0, r1);
 
         // ---- the item's end: sums across the warps, cell groups joined, rows written or left to be folded
 #pragma unroll
@@ -855,6 +902,16 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                 for (int z = 0; z < 4; ++z) acc[0][y][z] += __shfl_xor_sync(kFull, acc[0][y][z], 2);
             }
         }
+        auto write_out = [&](int64_t at, float4 o, float l) {   // sums o over the weights' sum l
+            const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+            o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+            if (p.gate != nullptr) {
+                const float4 v = __ldg(reinterpret_cast<const float4 *>(p.gate + at));
+                o.x = __fdiv_rn(o.x, 1.0f + expf(-v.x)), o.y = __fdiv_rn(o.y, 1.0f + expf(-v.y));
+                o.z = __fdiv_rn(o.z, 1.0f + expf(-v.z)), o.w = __fdiv_rn(o.w, 1.0f + expf(-v.w));
+            }
+            *reinterpret_cast<float4 *>(p.out + at) = o;
+        };
         float4 * s_red = reinterpret_cast<float4 *>(smem + G::red);
         if (cg > 0) {
 #pragma unroll
@@ -892,14 +949,10 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                     float4 o = make_float4(acc[x][0][z], acc[x][0][z + 2], acc[x][1][z], acc[x][1][z + 2]);
                     if (whole) {
                         const int64_t at = (int64_t(c.x.row0 + i) * p.n_q + c.h * p.group + (col0 + col - i * p.group)) * HD + dg * 32 + 4 * g;
-                        const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-                        o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
-                        if (p.gate != nullptr) {
-                            const float4 v = __ldg(reinterpret_cast<const float4 *>(p.gate + at));
-                            o.x = __fdiv_rn(o.x, 1.0f + expf(-v.x)), o.y = __fdiv_rn(o.y, 1.0f + expf(-v.y));
-                            o.z = __fdiv_rn(o.z, 1.0f + expf(-v.z)), o.w = __fdiv_rn(o.w, 1.0f + expf(-v.w));
-                        }
-                        *reinterpret_cast<float4 *>(p.out + at) = o;
+                        write_out(at, o, l);
+                    } else if constexpr (SHARED) {   // where the tiles were
+                        *reinterpret_cast<float4 *>(smem + G::ring + (col * HD + dg * 32 + 4 * g) * 4) = o;
+                        if (dg == 0 && g == 0) *reinterpret_cast<float2 *>(smem + G::ring + G::kCols * HD * 4 + col * 8) = make_float2(s_mfin[col], l);
                     } else {
                         *reinterpret_cast<float4 *>(p.ws_acc + (slot * G::kCols + col) * HD + dg * 32 + 4 * g) = o;
                         if (dg == 0 && g == 0) *reinterpret_cast<float2 *>(p.ws_ml + (slot * G::kCols + col) * 2) = make_float2(s_mfin[col], l);
@@ -907,8 +960,48 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                 }
             }
         }
-        u += uint32_t(n_tiles);
-        if (u < u1) c.next_item(p);
+        if constexpr (SHARED) {
+            if (c.x.tiles > 1) {   // the same in all CTAs of the cluster
+                cluster_barrier();
+                const int share = 1 << p.share_shift, each = G::kCols * HD / 4 >> p.share_shift;   // vectors of the outputs a CTA joins
+                for (int at = rank * each + tid; at < (rank + 1) * each; at += G::kThreads) {
+                    const int col = at / (HD / 4), v = at % (HD / 4), i = row_of_col(col);
+                    if (i >= c.x.m) continue;
+                    float2 ml[kMaxShare];
+                    float4 a[kMaxShare];
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int o = 0; o < kMaxShare; ++o) {
+                        const uint32_t from = smem_of(ring, o & (share - 1));   // all loads at once: none waits for a branch
+                        ml[o] = ld_cluster2(from + uint32_t(G::kCols * HD * 4 + col * 8));
+                        a[o] = ld_cluster4(from + uint32_t(at * 16));
+                        top = fmaxf(top, ml[o].x);
+                    }
+                    const float base = top == -INFINITY ? 0.0f : top;
+                    float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int o = 0; o < kMaxShare; ++o) {
+                        if (o >= share) break;
+                        const float w = ex2(ml[o].x - base);
+                        sum = fmaf(ml[o].y, w, sum);
+                        o4.x = fmaf(a[o].x, w, o4.x), o4.y = fmaf(a[o].y, w, o4.y), o4.z = fmaf(a[o].z, w, o4.z), o4.w = fmaf(a[o].w, w, o4.w);
+                    }
+                    write_out((int64_t(c.x.row0 + i) * p.n_q + c.h * p.group + (col0 + col - i * p.group)) * HD + v * 4, o4, sum);
+                }
+                cluster_barrier();   // nobody reads this CTA's part any more
+            }
+            shared_item += gridDim.x >> p.share_shift;
+            if (shared_item >= total) return;
+            find(shared_item, 0);
+            __syncthreads();
+            u = 0, u1 = uint32_t(c.at_share(p, int(s_start[0]), s_start[1], rank));
+            load.start(p, c, u1, ring);
+            k_at = G::ring, v_at = G::ring + 2 * G::kUnitBytes;
+        } else {
+            u += uint32_t(n_tiles);
+            if (u < u1) c.next_item(p);
+        }
     }
 }
 
@@ -1029,13 +1122,13 @@ __global__ void __launch_bounds__(kFoldThreads) attend_paged_fold_kernel(const _
 }
 
 // ---- launch -------------------------------------------------------------------------------------------------------------
-template <int HD, int NT>
+template <int HD, int NT, bool SHARED>
 bool configure() {
     static std::atomic<bool> done[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
     if (!done[dev].load(std::memory_order_acquire)) {
-        if (cudaFuncSetAttribute(attend_paged_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, geo<HD, NT>::total) != cudaSuccess) {
+        if (cudaFuncSetAttribute(attend_paged_kernel<HD, NT, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, geo<HD, NT>::total) != cudaSuccess) {
             (void) cudaGetLastError();
             return false;
         }
@@ -1058,9 +1151,8 @@ int column_blocks(const fnb_attend_paged_args * a) {
     return a->head_dim == 256 && cols > 8 ? 2 : 1;
 }
 constexpr int kGrid = 2 * kSmCount;  // two CTAs an SM
-// Items of a few tiles stay whole: a CTA takes them from end to end, and there is nothing to fold.  Cut, a short item's
-// tiles run side by side, and the fold costs less than three tiles in a row (8 requests of up to 300 cells, 16 heads over 2
-// of 256: 10.3 us cut, 11.9 whole).
+// Many items of a tile or two stay whole: a CTA takes them from end to end, and there is nothing to fold.  (Cut, an item of
+// three tiles has them side by side, and the fold costs less than three tiles in a row.)
 constexpr int kWholeTiles = 2;
 bool whole_items(const fnb_attend_paged_args * a) { return int64_t(a->max_pages) * a->page_size <= kWholeTiles * 128; }
 size_t paged_workspace(const fnb_attend_paged_args * a) {
@@ -1083,6 +1175,29 @@ bool paged_shape_ok(const fnb_attend_paged_args * a) {
     return true;
 }
 
+template <int HD, int NT>
+int64_t expected_items(const fnb_attend_paged_args * a, const paged_params & p) {   // by max_rows, a hint: a wrong one costs time only
+    constexpr int kCols = geo<HD, NT>::kCols;
+    const int64_t blocks = (int64_t(a->max_rows > 0 ? a->max_rows : 1) * p.group + kCols - 1) / kCols;
+    return int64_t(a->n_req) * a->n_kv_heads * blocks;
+}
+// The shared form: short items, few enough that each can have a cluster at once.  As many CTAs as tiles where the grid
+// allows it, else the most that leave a CTA two tiles; items that are longer or more numerous go on the line.  Nothing is
+// left in memory and the second launch falls away (16 heads over 2 of 256, us, line against shared: 8 requests of up to 300
+// cells 10.4 and 8.1, 64 of up to 500 18.9 and 12.3, one of 1000 9.4 and 7.1, 16 of 2000 12.6 and 11.9; but 64 of 1000, four
+// tiles a CTA, 20.5 and 22).  Returns log2 of the CTAs, 0 for the line.
+template <int HD, int NT>
+int share_of(const paged_params & p, int64_t items) {
+    const int64_t tiles = (p.cells_max + geo<HD, NT>::kTile - 1) / geo<HD, NT>::kTile;
+    for (int shift = 1; shift <= 3; ++shift) {
+        if (tiles <= int64_t(1) << shift && items << shift <= kGrid) return shift;
+    }
+    for (int shift = 3; shift >= 1; --shift) {
+        if (tiles <= int64_t(2) << shift && items << shift <= kGrid) return shift;
+    }
+    return 0;
+}
+
 void launch_fold(void (*kernel)(paged_params, int), dim3 blocks, cudaStream_t s, const paged_params & p, int grid) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = blocks, cfg.blockDim = dim3(kFoldThreads), cfg.stream = s;
@@ -1095,9 +1210,26 @@ void launch_fold(void (*kernel)(paged_params, int), dim3 blocks, cudaStream_t s,
 
 template <int HD, int NT>
 int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStream_t s) {
-    if (!configure<HD, NT>()) return FNB_LAUNCH_FAILED;
-    const int grid = kGrid;
     constexpr int kCols = geo<HD, NT>::kCols;
+    const int64_t items = expected_items<HD, NT>(a, p);
+    p.share_shift = share_of<HD, NT>(p, items);
+    if (p.share_shift > 0) {
+        if (!configure<HD, NT, true>()) return FNB_LAUNCH_FAILED;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(unsigned(items < kGrid >> p.share_shift ? items : kGrid >> p.share_shift) << p.share_shift);
+        cfg.blockDim = dim3(unsigned(geo<HD, NT>::kThreads));
+        cfg.dynamicSmemBytes = geo<HD, NT>::total, cfg.stream = s;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = 1u << p.share_shift, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr, cfg.numAttrs = 2;
+        (void) cudaLaunchKernelEx(&cfg, attend_paged_kernel<HD, NT, true>, p);
+        return launch_status();
+    }
+    if (!configure<HD, NT, false>()) return FNB_LAUNCH_FAILED;
+    const int grid = kGrid;
     const size_t cols = kCols;
     const bool fold = !p.whole;
     if (fold) {
@@ -1106,12 +1238,10 @@ int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStre
         p.ws_acc = reinterpret_cast<float *>(ws + size_t(grid) * 32);
         p.ws_ml = p.ws_acc + size_t(grid) * 2 * cols * HD;
     }
-    launch_pdl(attend_paged_kernel<HD, NT>, grid, geo<HD, NT>::kThreads, geo<HD, NT>::total, s, p);
+    launch_pdl(attend_paged_kernel<HD, NT, false>, grid, geo<HD, NT>::kThreads, geo<HD, NT>::total, s, p);
     if (cudaPeekAtLastError() != cudaSuccess) return FNB_LAUNCH_FAILED;
     if (fold) {
-        // Few items of a long table: list them.  (The number of items goes by max_rows, a hint; a wrong one costs time only.)
-        const int64_t blocks = (int64_t(a->max_rows > 0 ? a->max_rows : 1) * p.group + cols - 1) / int64_t(cols);
-        const int64_t items = int64_t(a->n_req) * a->n_kv_heads * blocks;
+        // Few items of a long table: list them.
         const int64_t outputs = items * int64_t(cols), wave = kSmCount * 8;   // columns to fold; blocks that run at a time
         if (outputs * (HD / 32) <= wave && p.cells_max >= 64 * 128) {
             launch_fold(attend_paged_fold_kernel<HD, kCols, 8, true>, dim3(unsigned(items), unsigned(cols), HD / 32), s, p, grid);
@@ -1125,9 +1255,13 @@ int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStre
 }
 }  // namespace
 
+template <int HD, int NT>
+bool configure_both() {
+    return configure<HD, NT, false>() && configure<HD, NT, true>();
+}
 bool attend_paged_prepare_device() {
-    return configure<256, 0>() && configure<256, 1>() && configure<256, 2>() && configure<128, 0>() && configure<128, 1>() &&
-           configure<64, 1>();
+    return configure_both<256, 0>() && configure_both<256, 1>() && configure_both<256, 2>() && configure_both<128, 0>() &&
+           configure_both<128, 1>() && configure_both<64, 1>();
 }
 
 }  // namespace fnb
