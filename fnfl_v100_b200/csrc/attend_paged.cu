@@ -23,11 +23,13 @@
 //   per group of 32 dims and outputs per tile in rounded F32 (sums run through all tiles in the tensor core were four
 //   times further from 64 bits).  Softmax statistics are F32.
 //
-// Work split: a unit is a tile of 128 cells (256 of narrow heads) of one (request, KV head, block of query columns).  The units of all
-// requests form one line that is cut into equal pieces, one for each resident CTA, wherever the requests' borders fall:
-// one long request and many ragged ones both fill the machine, from lengths only the device knows.  A piece that holds
-// all tiles of an item writes its rows itself; otherwise it leaves its sums, maximum and accumulators in the workspace
-// and a second launch folds an item's pieces in their order.  Where a table lists few cells and there are few items, an
+// Work split: a unit is a tile of 128 cells (256 of narrow heads) of one (request, KV head, block of query columns), an
+// item, or an item's start: its queries, first copies and last sums cost about what a tile does, and a line of tiles alone
+// left the pieces with most items behind (64 requests of up to 8192 cells 64.7 us against 59.9; two units a start 62.2).
+// The units of all requests form one line that is cut into equal pieces, one for each resident CTA, wherever the requests'
+// borders fall: one long request and many ragged ones both fill the machine, from lengths only the device knows.  A piece
+// that holds all tiles of an item writes its rows itself; otherwise it leaves its sums, maximum and accumulators in the
+// workspace and a second launch folds an item's pieces in their order.  Where a table lists few cells and there are few items, an
 // item's tiles go to a cluster of CTAs instead, which join their parts through shared memory (share_of).  Results do not
 // depend on timing.
 //
@@ -41,8 +43,8 @@
 // scheduler.  The change took 61 us to 50 at 196 608 cells.)
 //
 // Measured on a B200, graph replays over caches larger than L2: one request of 196 608 cells, 16 heads over 2 of 256:
-// 43.2 us, 113 MB at 2.6 TB/s; 40 requests of up to 5000 cells, 32 heads over 8 of 128: 51 us; 8 requests of up to 300
-// cells: 8.1 us, latency.  In its steady state a warp issues some 790 instructions a tile at 0.56 to 0.6 an issue slot,
+// 43.2 us, 113 MB at 2.6 TB/s; 40 requests of up to 5000 cells, 32 heads over 8 of 128: 45 us; 8 requests of up to 300
+// cells: 7.9 us, latency.  In its steady state a warp issues some 790 instructions a tile at 0.56 to 0.6 an issue slot,
 // the logic, FP16 and tensor units each 35 to 40 % busy; cells that lie in L2 give the same time.
 #include <atomic>
 #include <type_traits>
@@ -55,6 +57,7 @@ namespace {
 
 constexpr int kMaxReq = 2048;
 constexpr float kLog2eF = 1.4426950408889634f;
+constexpr int kStart = 1;                        // units that an item's start counts
 constexpr int kMaxShare = 8;                     // CTAs that share an item in the clustered form, at most
 constexpr float kPShift = 14.0f;                 // probabilities are held times 2^14
 
@@ -230,7 +233,7 @@ __device__ __forceinline__ request load_request(const paged_params & p, int r, b
 }
 template <bool ITEMS>
 __device__ __forceinline__ int64_t units_of(const paged_params & p, const request & x) {  // or its items
-    return int64_t(p.n_kv) * x.blocks * (ITEMS ? 1 : x.tiles);
+    return int64_t(p.n_kv) * x.blocks * (ITEMS ? 1 : x.tiles + kStart);
 }
 
 // the walk over a piece of the line: request, KV head, column block, tile
@@ -238,11 +241,12 @@ template <class G>
 struct cursor {
     int r, h, blk, tile;
     request x;
+    // unit `offset` of the request: an item is its start, kStart units below 0 here, and then its tiles
     __device__ __forceinline__ void at(const paged_params & p, int request_index, uint32_t offset) {
         r = request_index;
         x = load_request<G>(p, r, false);
-        const uint32_t item = offset / uint32_t(x.tiles);
-        tile = int(offset - item * uint32_t(x.tiles));
+        const uint32_t item = offset / uint32_t(x.tiles + kStart);
+        tile = int(offset - item * uint32_t(x.tiles + kStart)) - kStart;
         h = int(item / uint32_t(x.blocks));
         blk = int(item - uint32_t(h) * uint32_t(x.blocks));
     }
@@ -295,7 +299,8 @@ struct loader {
     static constexpr int kCh = G::kGroups, kRows = 32 / kCh, kPass = 16 / kRows, kRow = HD / 2, kScale = kCh * 2;
     static constexpr int kLag = 4 - G::kVStages, S = G::kSets;  // a tile is S sets of 128 rows, sixteen to a warp
     cursor<G> c;
-    uint32_t step, tiles;     // of the piece
+    uint32_t step, last;      // steps so far; behind the piece's last tile
+    int units;                // of the piece from this tile on
     uint32_t k_st, v_st;      // where the next copies go
     int32_t id[S];            // pages of the warp's rows in tile `step`
     uint32_t cell[kLag][S];   // first of its rows in the kLag tiles before `step` (the last first), counted through all heads of a plane
@@ -311,8 +316,8 @@ struct loader {
             id[q] = at < c.x.n ? __ldg(t + (at >> p.page_shift)) : 0;
         }
     }
-    __device__ __forceinline__ void start(const paged_params & p, const cursor<G> & from, uint32_t n, uint32_t ring) {
-        c = from, step = 0, tiles = n, k_st = ring, v_st = ring + 2 * G::kUnitBytes;
+    __device__ __forceinline__ void start(const paged_params & p, const cursor<G> & from, int n, uint32_t ring) {
+        c = from, step = 0, units = n, last = n > 0 ? 0xffffff00u : 0u, k_st = ring, v_st = ring + 2 * G::kUnitBytes;
 #pragma unroll
         for (int i = 0; i < kLag; ++i) {
             left[i] = 0;
@@ -345,8 +350,8 @@ struct loader {
                            (lower ? p.k_scale : p.v_scale) + uint64_t(at) * kCh, ALL || int(lane & 15) < (lower ? k_some : v_some));
     }
     __device__ __forceinline__ void next(const paged_params & p, uint32_t ring) {
-        if (step >= tiles + kLag) return;
-        const bool k_too = step < tiles, v_too = step >= uint32_t(kLag);
+        if (step >= last + kLag) return;
+        const bool k_too = step < last, v_too = step >= uint32_t(kLag);
         const int base = c.tile * G::kTile + warp_row(), k_left = c.x.n - base, v_left = left[kLag - 1];
         const uint32_t head = uint32_t(c.h) * uint32_t(p.cache_slots), mask = (1u << p.page_shift) - 1;
         uint32_t k_cell[S];
@@ -389,11 +394,17 @@ struct loader {
         left[0] = k_left;
 #pragma unroll
         for (int q = 0; q < S; ++q) cell[0][q] = k_cell[q];
-        if (step + 1 < tiles) {
-            if (++c.tile >= c.x.tiles) c.next_item(p);
-            fetch(p);
-        }
         ++step;
+        if (k_too) {
+            --units;
+            if (++c.tile >= c.x.tiles) units -= kStart;
+            if (units > 0) {
+                if (c.tile >= c.x.tiles) c.next_item(p);
+                fetch(p);
+            } else {
+                last = step;
+            }
+        }
         k_st = step & 1 ? ring + G::kUnitBytes : ring;
         if (v_too) v_st = v_st == ring + (G::kStages - 1) * G::kUnitBytes ? ring + 2 * G::kUnitBytes : v_st + G::kUnitBytes;
     }
@@ -472,11 +483,17 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
     if (!SHARED && p.whole && u0 < u1) {
         cursor<G> at;
         at.at(p, int(s_start[0]), s_start[1]);
-        u0 -= uint32_t(at.tile);
+        u0 -= uint32_t(at.tile + kStart);
         if (u1 < total) {
             at.at(p, int(s_start[2]), s_start[3]);
-            u1 -= uint32_t(at.tile);
+            u1 -= uint32_t(at.tile + kStart);
         }
+    }
+    cursor<G> c;
+    if (!SHARED && u0 < u1) {
+        c.at(p, int(s_start[0]), s_start[1]);
+        if (p.whole) c.tile = -kStart;
+        if (c.tile < 0) u0 += uint32_t(-c.tile), c.tile = 0;   // nothing to do there
     }
     if (u0 >= u1) {
         if (tid == 0 && p.ws_head != nullptr) {
@@ -484,16 +501,12 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
         }
         return;
     }
-    cursor<G> c;
     if constexpr (SHARED) {
         u1 = uint32_t(c.at_share(p, int(s_start[0]), s_start[1], rank));
-    } else {
-        c.at(p, int(s_start[0]), s_start[1]);
-        if (p.whole) c.tile = 0;
     }
     const uint32_t ring = smem_u32(smem) + G::ring;
     loader<G, HD> load;
-    load.start(p, c, u1 - u0, ring);
+    load.start(p, c, int(u1 - u0), ring);
     if (!SHARED && tid == G::kThreads - 1 && p.ws_head != nullptr) {
         fold_head f = {0, 0, 0, c.h, c.blk, c.x.row0, c.x.m, 0};
         if (c.tile != 0) {
@@ -996,10 +1009,10 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
             find(shared_item, 0);
             __syncthreads();
             u = 0, u1 = uint32_t(c.at_share(p, int(s_start[0]), s_start[1], rank));
-            load.start(p, c, u1, ring);
+            load.start(p, c, int(u1), ring);
             k_at = G::ring, v_at = G::ring + 2 * G::kUnitBytes;
         } else {
-            u += uint32_t(n_tiles);
+            u += uint32_t(n_tiles + kStart);
             if (u < u1) c.next_item(p);
         }
     }

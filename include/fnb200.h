@@ -466,7 +466,7 @@ int32_t fnb_attend_static(const fnb_attend_args * args, void * stream);
  * head_dim 64, 128 or 256; n_req in [1, 2048]; page_size a power of two from 16 to 2^20; cache_slots a multiple of it
  * below 2^31, cache_slots n_kv_heads below 2^32; n_q_heads a multiple of n_kv_heads up to 1024, rows n_q_heads below 2^31;
  * q, gate, out, caches and scales 16-byte aligned.  out may not overlap an input.  The tiles to visit (128 cells, 256 when
- * head_dim is below 256; times passes and KV heads, over all requests) number below 2^31: else FNB_ERR_PAGES, nothing written.
+ * head_dim is below 256, and one more a request; times passes and KV heads) number below 2^31: else FNB_ERR_PAGES, nothing written.
  * workspace: at least fnb_attend_paged_workspace_bytes(args) bytes (a function of head_dim, max_rows, the head counts
  * and whether max_pages page_size exceeds 256, not of the lengths; up to 256 none is needed and null is taken), 16-byte
  * aligned; its contents need no initialisation and mean nothing afterwards.  Calls that share a workspace must not overlap on the GPU.
