@@ -70,7 +70,7 @@ class AttendPagedArgs(C.Structure):
                 ("row_start", C.c_void_p), ("out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
                 ("err", C.c_void_p), ("cache_slots", C.c_int64), ("rows", C.c_int32), ("n_req", C.c_int32),
                 ("max_pages", C.c_int32), ("page_size", C.c_int32), ("max_rows", C.c_int32), ("n_q_heads", C.c_int32),
-                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("scale", C.c_float)]
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("scale", C.c_float), ("table_stride", C.c_int32)]
 
 
 class GgufTensor(C.Structure):

@@ -111,7 +111,7 @@ struct paged_params {
     uint32_t * err;
     int64_t cache_slots;
     int cells_max;      // what a table row can list
-    int rows, n_req, max_pages, n_pages, page_shift, n_q, n_kv, group;
+    int rows, n_req, table_stride, n_pages, page_shift, n_q, n_kv, group;
     float scale_log2;
     uint32_t e1024, e64;  // FP16 exponents, twice each (code_low, code_high)
     // n / group = n group_mul >> group_shift for n < 2^31: group_mul = floor(2^(31 + l) / group) + 1 with 2^l >= group is off by
@@ -309,7 +309,7 @@ struct loader {
 
     __device__ __forceinline__ static int warp_row() { return int(threadIdx.x >> 5) * 16; }
     __device__ __forceinline__ void fetch(const paged_params & p) {
-        const int32_t * t = p.table + int64_t(c.r) * p.max_pages;
+        const int32_t * t = p.table + int64_t(c.r) * p.table_stride;
 #pragma unroll
         for (int q = 0; q < S; ++q) {
             const int at = c.tile * G::kTile + q * 128 + warp_row();
@@ -1179,6 +1179,7 @@ bool paged_shape_ok(const fnb_attend_paged_args * a) {
     if (a == nullptr) return false;
     if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return false;
     if (a->rows < 1 || a->n_req < 1 || a->n_req > kMaxReq || a->max_pages < 1 || a->max_rows < 0) return false;
+    if (a->table_stride != 0 && a->table_stride < a->max_pages) return false;
     if (a->row_start == nullptr && a->rows < a->n_req) return false;
     if (int64_t(a->rows) * a->n_q_heads > INT32_MAX) return false;
     if (a->n_q_heads < 1 || a->n_kv_heads < 1 || a->n_q_heads > 1024 || a->n_q_heads % a->n_kv_heads != 0) return false;
@@ -1297,7 +1298,8 @@ extern "C" int32_t fnb_attend_paged_kv4(const fnb_attend_paged_args * a, void * 
     p.k_cache = static_cast<const uint8_t *>(a->k_cache), p.v_cache = static_cast<const uint8_t *>(a->v_cache);
     p.q = a->q, p.gate = a->gate, p.k_scale = a->k_scale, p.v_scale = a->v_scale;
     p.table = a->table, p.n_cells = a->n_cells, p.row_start = a->row_start, p.out = a->out, p.err = a->err;
-    p.cache_slots = a->cache_slots, p.rows = a->rows, p.n_req = a->n_req, p.max_pages = a->max_pages;
+    p.cache_slots = a->cache_slots, p.rows = a->rows, p.n_req = a->n_req;
+    p.table_stride = a->table_stride != 0 ? a->table_stride : a->max_pages;
     const int64_t held = int64_t(a->max_pages) * a->page_size;
     p.cells_max = int(held < INT32_MAX - 256 ? held : INT32_MAX - 256);
     p.n_pages = int(a->cache_slots / a->page_size), p.page_shift = __builtin_ctz(unsigned(a->page_size));

@@ -421,16 +421,22 @@ def attend_paged_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      workspace: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q [rows][n_q][hd] over the paged KV4 cache: request r's rows are row_start[r] .. row_start[r + 1] - 1 (None:
     one row a request) and see its n_cells[r] cells, the pages table[r] lists, causally.  max_rows: the most rows of a request
-    (a hint).  Rows of no request are left as they were in `out`, which may not overlap an input.  `workspace` (uint8) is used
+    (a hint).  `table` may be the first columns of a wider one (table[:, :w], once no request has more pages): narrow tables are
+    served faster.  Rows of no request are left as they were in `out`, which may not overlap an input.  `workspace` (uint8) is used
     when it is large enough, else one is allocated.  Returns out [rows][n_q][hd]."""
     _dev(q, torch.float32, "q")
     n_kv, slots, hd = _kv4_planes(k_cache, k_scale, "k")
     if q.dim() != 3 or q.shape[2] != hd or _kv4_planes(v_cache, v_scale, "v") != (n_kv, slots, hd):
         raise ValueError("q: expected [rows][n_q_heads][head_dim]; k_cache / v_cache: planes of new_kv_cache for this head_dim")
-    _dev(table, torch.int32, "table")
-    if table.dim() != 2:
-        raise ValueError("table: expected [n_req][max_pages]")
+    if not (isinstance(table, torch.Tensor) and table.is_cuda and table.dtype == torch.int32 and table.dim() == 2):
+        raise ValueError("table: expected a CUDA tensor [n_req][max_pages] of torch.int32")
     n_req, max_pages = table.shape
+    stride = 0
+    if not table.is_contiguous():
+        stride, one = table.stride()
+        if (one != 1 and max_pages > 1) or (stride < max_pages and n_req > 1) or stride > 2**31 - 1:
+            raise ValueError("table: expected rows of consecutive entries")
+        stride = max(stride, max_pages)
     _numel(_dev(n_cells, torch.int32, "n_cells"), n_req, "n_cells")
     if row_start is not None:
         _numel(_dev(row_start, torch.int32, "row_start"), n_req + 1, "row_start")
@@ -444,7 +450,7 @@ def attend_paged_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         a = _lib.AttendPagedArgs(q.data_ptr(), _at(gate), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                  table.data_ptr(), n_cells.data_ptr(), _at(row_start), out.data_ptr(), None, 0, _at(err), slots,
                                  q.shape[0], n_req, max_pages, page_size, max_rows, q.shape[1], n_kv, hd,
-                                 hd ** -0.5 if scale is None else float(scale))
+                                 hd ** -0.5 if scale is None else float(scale), stride)
         need = _lib.lib().fnb_attend_paged_workspace_bytes(C.byref(a))
         if need == 0:
             raise ValueError("attend_paged_kv4: shape outside the contract")

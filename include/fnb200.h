@@ -197,7 +197,8 @@ int32_t fnb_rope_neox_kv8_append(const fnb_rope_kv8_args * args, void * stream);
  * v_cache uint8 [n_kv_heads][cache_slots][head_dim / 2], two codes a byte in the order of the values, low nibble first;
  * k_scale / v_scale FP16 [n_kv_heads][cache_slots][head_dim / 32], 16-byte aligned.  144 bytes a 256-wide cell where
  * Q8_0 takes 272 and KV8 264.  A slot of -1 marks a row of padding: nothing is written for it and no fault is flagged
- * (fnb_page_tables writes such slots).  Everything else as fnb_rope_neox_kv8_append.  The reference has no 4-bit cache.
+ * (fnb_page_tables writes such slots).  The other slots of a call must differ: a cell given twice may end with the codes
+ * of one row and the scales of the other.  Everything else as fnb_rope_neox_kv8_append.  The reference has no 4-bit cache.
  */
 int32_t fnb_rope_neox_kv4_append(const fnb_rope_kv8_args * args, void * stream);
 
@@ -455,7 +456,10 @@ int32_t fnb_attend_static(const fnb_attend_args * args, void * stream);
  * are its last cells: row i of m sees the first n_cells[r] - m + i + 1 of them (causal).  All three arrays are read on
  * the device, so one captured graph serves every step; fnb_page_tables writes them.  A row that sees no cell gives
  * zeros; rows that belong to no request are left as they were.  What lies in a page behind a request's last cell, or in
- * cells a row does not see, does not touch its result, NaN included.
+ * cells a row does not see, does not touch its result, NaN included.  Requests may share pages.
+ * How the work is split goes by max_pages (and n_req, max_rows, the heads), since lengths are the device's: tables of few
+ * cells, up to 2048 a request (4096 when head_dim is below 256), are served faster.  A caller that keeps wide tables may
+ * give the first columns of one, max_pages of them in rows table_stride apart, once no request is longer.
  * max_rows (a hint; 0 means 1): the most rows a request has.  The query columns of a KV head (rows x n_q_heads /
  * n_kv_heads) are served eight to a pass over its cells (four when max_rows gives no more and head_dim is at least 128,
  * sixteen when it gives more than eight and head_dim is 256); more columns are more passes, read mostly from L2.  A wrong hint costs time, not results.
@@ -497,6 +501,7 @@ typedef struct fnb_attend_paged_args {
     int32_t n_kv_heads;
     int32_t head_dim;
     float scale;
+    int32_t table_stride; /* entries from one request's row of the table to the next; 0: max_pages */
 } fnb_attend_paged_args;
 
 size_t fnb_attend_paged_workspace_bytes(const fnb_attend_paged_args * args); /* 0 for a shape outside the contract */

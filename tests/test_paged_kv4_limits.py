@@ -41,3 +41,12 @@ def test_workspace_is_needed_only_where_items_are_cut(lib):
     small = {size(max_pages=16), size(max_pages=1), size(max_pages=2, page_size=128), size(max_pages=16, max_rows=9)}
     assert len(small) == 1 and 0 < small.pop() <= 256
     assert size(max_pages=17) == size(max_pages=1 << 20) < size(max_pages=17, max_rows=2)
+
+
+def test_table_stride(lib):
+    """0 stands for max_pages; less than max_pages is refused."""
+    for stride, ok in ((0, True), (100, True), (5000, True), (99, False), (-1, False), (-100, False)):
+        a = _lib.AttendPagedArgs(**{**SHAPE, "table_stride": stride})
+        assert (lib.fnb_attend_paged_workspace_bytes(C.byref(a)) > 0) == ok
+        if not ok:
+            assert lib.fnb_attend_paged_kv4(C.byref(a), None) == _lib.REJECTED
