@@ -43,8 +43,8 @@
 // scheduler.  The change took 61 us to 50 at 196 608 cells.)
 //
 // Measured on a B200, graph replays over caches larger than L2: one request of 196 608 cells, 16 heads over 2 of 256:
-// 43.2 us, 113 MB at 2.6 TB/s; 40 requests of up to 5000 cells, 32 heads over 8 of 128: 45 us; 8 requests of up to 300
-// cells: 7.9 us, latency.  In its steady state a warp issues some 790 instructions a tile at 0.56 to 0.6 an issue slot,
+// 43.2 us, 113 MB at 2.6 TB/s; 40 requests of up to 5000 cells, 32 heads over 8 of 128: 43 us; 8 requests of up to 300
+// cells: 7.5 us, latency.  In its steady state a warp issues some 790 instructions a tile at 0.56 to 0.6 an issue slot,
 // the logic, FP16 and tensor units each 35 to 40 % busy; cells that lie in L2 give the same time.
 #include <atomic>
 #include <type_traits>
@@ -1022,17 +1022,21 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
 // One column, VEC float4 vectors of dims a block, the other threads split the pieces: weights 2^(m - max), accumulators
 // and sums joined in the order of the pieces.  LISTED: block k takes the k-th, (k + gridDim.x)-th .. of the cut items,
 // found by listing the pieces' marks (few items, each in many pieces: few blocks an item would leave most of the machine
-// idle).  Else block k looks at piece k + 1 alone, which costs one load where there is nothing to fold.
+// idle); all weights are made first, from maxima in shared memory.  Else block k looks at piece k + 1 alone, which costs one
+// load where there is nothing to fold, and as its items lie in few pieces each thread joins its own as they arrive (40
+// requests of up to 5000 cells, 320 items: 43.1 us against 44.9; items in ten pieces or more lose 1 to 2 us that way).
 constexpr int kFoldThreads = 256;
 constexpr int kMaxPieces = 2 * kSmCount;
 template <int HD, int COLS, int VEC, bool LISTED>
 __global__ void __launch_bounds__(kFoldThreads) attend_paged_fold_kernel(const __grid_constant__ paged_params p, const int pieces_all) {
     constexpr int SPLIT = kFoldThreads / VEC;
     __shared__ float4 s_acc[SPLIT][VEC];
-    __shared__ float s_max[kFoldThreads / 32], s_sum[kFoldThreads / 32];
-    __shared__ float s_weight[kMaxPieces], s_part[kMaxPieces];
-    __shared__ fold_head s_head[LISTED ? kMaxPieces : 1];
-    __shared__ int s_count[2 * kFoldThreads / 32];
+    [[maybe_unused]] __shared__ float s_max[kFoldThreads / 32], s_sum[kFoldThreads / 32];
+    [[maybe_unused]] __shared__ float s_weight[LISTED ? kMaxPieces : 1], s_part[LISTED ? kMaxPieces : 1];
+    [[maybe_unused]] __shared__ fold_head s_head[LISTED ? kMaxPieces : 1];
+    [[maybe_unused]] __shared__ int s_count[2 * kFoldThreads / 32];
+    constexpr int JOINED = VEC < 32 ? kFoldThreads / 32 : SPLIT;   // parts left once a warp has joined its own
+    [[maybe_unused]] __shared__ float2 s_ml[JOINED];
     static_assert(kMaxPieces <= 2 * kFoldThreads, "two heads a thread");
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, col = blockIdx.y;
@@ -1078,53 +1082,105 @@ __global__ void __launch_bounds__(kFoldThreads) attend_paged_fold_kernel(const _
         // The pieces after the first hold the item from their start: slot 0; in the first it is the last: slot 1.
         const int n = f.to - f.from + 1;
         auto slot_of = [&](int j) { return (int64_t(f.from + j) * 2 + (j == 0 ? 1 : 0)) * COLS + col; };
-        // the first pieces' accumulators are on their way before the weights are known
         const int v = tid % VEC, part = tid / VEC;
-        auto acc_of = [&](int j) { return __ldcg(reinterpret_cast<const float4 *>(p.ws_acc + slot_of(j) * HD) + blockIdx.z * VEC + v); };
-        constexpr int kAhead = 4;
-        float4 ahead[kAhead];
+        float a = 0.0f, s = 0.0f;   // a dim's sum and the weights', in the first VEC * 4 threads
+        if constexpr (LISTED) {
+            // the first pieces' accumulators are on their way before the weights are known
+            auto acc_of = [&](int j) { return __ldcg(reinterpret_cast<const float4 *>(p.ws_acc + slot_of(j) * HD) + blockIdx.z * VEC + v); };
+            constexpr int kAhead = 4;
+            float4 ahead[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) ahead[i] = part + i * SPLIT < n ? acc_of(part + i * SPLIT) : make_float4(0.f, 0.f, 0.f, 0.f);
-        float top = -INFINITY;
-        for (int j = tid; j < n; j += kFoldThreads) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.ws_ml + slot_of(j) * 2));
-            s_weight[j] = ml.x, s_part[j] = ml.y;
-            top = fmaxf(top, ml.x);
-        }
+            for (int i = 0; i < kAhead; ++i) ahead[i] = part + i * SPLIT < n ? acc_of(part + i * SPLIT) : make_float4(0.f, 0.f, 0.f, 0.f);
+            float top = -INFINITY;
+            for (int j = tid; j < n; j += kFoldThreads) {
+                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.ws_ml + slot_of(j) * 2));
+                s_weight[j] = ml.x, s_part[j] = ml.y;
+                top = fmaxf(top, ml.x);
+            }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-        if (lane == 0) s_max[wid] = top;
-        __syncthreads();
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+            if (lane == 0) s_max[wid] = top;
+            __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kFoldThreads / 32; ++w) top = fmaxf(top, s_max[w]);
-        const float base = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f;
-        for (int j = tid; j < n; j += kFoldThreads) {
-            const float w = ex2(s_weight[j] - base);
-            s_weight[j] = w;
-            sum = fmaf(s_part[j], w, sum);
-        }
+            for (int w = 0; w < kFoldThreads / 32; ++w) top = fmaxf(top, s_max[w]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f;
+            for (int j = tid; j < n; j += kFoldThreads) {
+                const float w = ex2(s_weight[j] - base);
+                s_weight[j] = w;
+                sum = fmaf(s_part[j], w, sum);
+            }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-        if (lane == 0) s_sum[wid] = sum;
-        __syncthreads();
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto join = [&](float4 a, float w) {
-            acc.x = fmaf(a.x, w, acc.x), acc.y = fmaf(a.y, w, acc.y), acc.z = fmaf(a.z, w, acc.z), acc.w = fmaf(a.w, w, acc.w);
-        };
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+            if (lane == 0) s_sum[wid] = sum;
+            __syncthreads();
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto join = [&](float4 a, float w) {
+                acc.x = fmaf(a.x, w, acc.x), acc.y = fmaf(a.y, w, acc.y), acc.z = fmaf(a.z, w, acc.z), acc.w = fmaf(a.w, w, acc.w);
+            };
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            if (part + i * SPLIT < n) join(ahead[i], s_weight[part + i * SPLIT]);
-        }
+            for (int i = 0; i < kAhead; ++i) {
+                if (part + i * SPLIT < n) join(ahead[i], s_weight[part + i * SPLIT]);
+            }
 #pragma unroll 8
-        for (int j = part + kAhead * SPLIT; j < n; j += SPLIT) join(acc_of(j), s_weight[j]);
-        s_acc[part][v] = acc;
-        __syncthreads();
-        if (tid < VEC * 4) {
-            float a = 0.0f, s = 0.0f;
-            for (int o = 0; o < min(SPLIT, n); ++o) a += reinterpret_cast<const float *>(s_acc[o])[tid];
+            for (int j = part + kAhead * SPLIT; j < n; j += SPLIT) join(acc_of(j), s_weight[j]);
+            s_acc[part][v] = acc;
+            __syncthreads();
+            if (tid < VEC * 4) {
+                for (int o = 0; o < min(SPLIT, n); ++o) a += reinterpret_cast<const float *>(s_acc[o])[tid];
 #pragma unroll
-            for (int w = 0; w < kFoldThreads / 32; ++w) s += s_sum[w];
+                for (int w = 0; w < kFoldThreads / 32; ++w) s += s_sum[w];
+            }
+        } else {
+            // a thread's pieces: maximum, sum and accumulators so far, brought to a common maximum as each is joined
+            float top = -INFINITY, sum = 0.0f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto join = [&](float2 ml, float4 x) {
+                const float t = fmaxf(top, ml.x), base = t == -INFINITY ? 0.0f : t;
+                const float w0 = ex2(top - base), w1 = ex2(ml.x - base);
+                top = t, sum = fmaf(ml.y, w1, sum * w0);
+                acc.x = fmaf(x.x, w1, acc.x * w0), acc.y = fmaf(x.y, w1, acc.y * w0), acc.z = fmaf(x.z, w1, acc.z * w0), acc.w = fmaf(x.w, w1, acc.w * w0);
+            };
+            constexpr int kAhead = 4;
+            for (int j = part; j < n; j += kAhead * SPLIT) {
+                float2 ml[kAhead];
+                float4 x[kAhead];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    ml[i] = make_float2(-INFINITY, 0.0f), x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (j + i * SPLIT >= n) continue;
+                    const int64_t at = slot_of(j + i * SPLIT);
+                    ml[i] = __ldcg(reinterpret_cast<const float2 *>(p.ws_ml + at * 2));
+                    x[i] = __ldcg(reinterpret_cast<const float4 *>(p.ws_acc + at * HD) + blockIdx.z * VEC + v);
+                }
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) join(ml[i], x[i]);
+            }
+            if constexpr (VEC < 32) {
+#pragma unroll
+                for (int o = VEC; o < 32; o <<= 1) {
+                    const float2 ml = make_float2(__shfl_xor_sync(kFull, top, o), __shfl_xor_sync(kFull, sum, o));
+                    join(ml, make_float4(__shfl_xor_sync(kFull, acc.x, o), __shfl_xor_sync(kFull, acc.y, o), __shfl_xor_sync(kFull, acc.z, o),
+                                         __shfl_xor_sync(kFull, acc.w, o)));
+                }
+            }
+            const int joined = VEC < 32 ? wid : part;
+            if (VEC >= 32 || lane < VEC) s_acc[joined][v] = acc;
+            if (VEC >= 32 ? v == 0 : lane == 0) s_ml[joined] = make_float2(top, sum);
+            __syncthreads();
+            if (tid < VEC * 4) {
+                float t = -INFINITY;
+#pragma unroll
+                for (int o = 0; o < JOINED; ++o) t = fmaxf(t, s_ml[o].x);
+                const float base = t == -INFINITY ? 0.0f : t;
+#pragma unroll
+                for (int o = 0; o < JOINED; ++o) {
+                    const float w = ex2(s_ml[o].x - base);
+                    a = fmaf(reinterpret_cast<const float *>(s_acc[o])[tid], w, a), s = fmaf(s_ml[o].y, w, s);
+                }
+            }
+        }
+        if (tid < VEC * 4) {
             float y = s == 0.0f ? 0.0f : __fdiv_rn(a, s);
             const int64_t at = (int64_t(f.row0 + row) * p.n_q + f.h * p.group + (f.blk * COLS + col - row * p.group)) * HD + blockIdx.z * VEC * 4 + tid;
             if (p.gate != nullptr) y = __fdiv_rn(y, 1.0f + expf(-__ldg(p.gate + at)));
