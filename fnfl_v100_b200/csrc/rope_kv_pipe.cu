@@ -410,9 +410,12 @@ bool launch_one(const rope_kernel_args & a, cudaStream_t s) {
         return st;
     };
     // Tokens a tile: a group's warps take four rows each at a time, so the rows of a tile should fill whole rounds of them;
-    // of the sizes that do so best, among those that leave the ring its full depth, the smallest.
+    // of the sizes that do so best, among those that leave the ring its full depth, the smallest.  Tiles of more than one
+    // token only where every SM has one: a token's angles are most of a small call's time (64 tokens of
+    // 8 + 1 + 1 heads of 256: 4.0 us, in tiles of four 5.7; of 16 + 4 + 4 of 128: 3.5, in tiles of five 4.8).
+    const int64_t most = a.rows / kSmCount < 1 ? 1 : a.rows / kSmCount < kMaxTile ? a.rows / kSmCount : kMaxTile;
     int tt = 1, stages = fit(1), best = 0;
-    for (int t = 1; t <= kMaxTile; ++t) {
+    for (int t = 1; t <= most; ++t) {
         const int st = fit(t), quads = (t * rpt + 3) / 4, rounds = (quads + kGroupWarps - 1) / kGroupWarps;
         const int filled = t * rpt * 25 / (rounds * kGroupWarps);  // per cent
         if (st == stages && filled > best + 2) tt = t, best = filled;
