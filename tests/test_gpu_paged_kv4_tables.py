@@ -54,3 +54,16 @@ def test_requests_share_pages(dev):
         err = ops.new_err(dev)
         got = ops.attend_paged_kv4(to_dev(q, dev), *planes, to_dev(wide, dev), to_dev(np.array(lens, np.int32), dev), page_size=page, err=err)
         assert int(err.item()) == 0 and (np.abs(got.cpu().numpy() - ref) <= tol).all(), width
+
+
+def test_more_tiles_than_the_line_counts(dev):
+    """Lengths that are valid one by one but make 2^31 tiles or more together: flagged, nothing read or written."""
+    n_req, page = 400, 1 << 20
+    kc, ks = ops.new_kv_cache(page, 1, 64, dev, fmt="kv4")
+    table = torch.zeros((n_req, 2047), dtype=torch.int32, device=dev)
+    lens = torch.full((n_req,), 2047 * page, dtype=torch.int32, device=dev)
+    q = torch.ones((n_req, 8, 64), device=dev)
+    out, err = torch.full_like(q, 9.0), ops.new_err(dev)
+    ops.attend_paged_kv4(q, kc, kc, ks, ks, table, lens, page_size=page, out=out, err=err)
+    torch.cuda.synchronize()
+    assert int(err.item()) == ops.ERR_PAGES and bool((out == 9.0).all())
