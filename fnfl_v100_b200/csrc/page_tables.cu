@@ -19,7 +19,7 @@ namespace {
 constexpr int kThreadsT = 1024;
 constexpr int kMaxRequests = 2048;
 constexpr int kPerThread = kMaxRequests / kThreadsT;
-constexpr int kRowsOneCta = 4096;
+constexpr int kRowsOneCta = 1024;  // 4096 rows: one CTA 7.2 us, eight 5.2
 constexpr int kClusterCtas = 8;
 
 struct tables_params {
@@ -69,6 +69,8 @@ __device__ __forceinline__ int owner_of(const int32_t * end, int n, int64_t i) {
     return lo;
 }
 
+// ROWS: neighbouring rows a thread takes at a time, 1 or 4
+template <int ROWS>
 __global__ void __launch_bounds__(kThreadsT) page_tables_kernel(const tables_params p) {
     __shared__ int64_t s_warp[32];
     __shared__ int32_t s_row_end[kMaxRequests], s_page_end[kMaxRequests];
@@ -149,28 +151,50 @@ __global__ void __launch_bounds__(kThreadsT) page_tables_kernel(const tables_par
         const int64_t j = i - (r > 0 ? int64_t(s_page_end[r - 1]) : 0);
         p.table[int64_t(r) * p.max_pages + held + j] = __ldg(p.free_pages + head + i);
     }
-    // rows; a page of this step is read off the free list, not from the table another thread is filling
+    // Rows; a page of this step is read off the free list, not from the table another thread is filling.  Neighbours mostly
+    // share request and page, and so one search and one dependent load.
     const int64_t n_rows = s_row_end[n_req - 1];
-    for (int64_t i = first; i < p.rows; i += step) {
-        int32_t slot = -1, at_pos = -1;
-        if (i < n_rows) {
-            const int r = owner_of(s_row_end, n_req, i);
+    for (int64_t i0 = first * ROWS; i0 < p.rows; i0 += step * ROWS) {
+        int32_t slot[ROWS], at_pos[ROWS];
+        int r = -1;
+        int64_t page_of = -1;   // the page that `id` belongs to
+        int32_t id = -1;
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+            const int64_t i = i0 + k;
+            slot[k] = -1, at_pos[k] = -1;
+            if (i >= n_rows) continue;
+            if (r < 0 || i >= s_row_end[r]) r = owner_of(s_row_end, n_req, i), page_of = -1;
             const int64_t o = s_old[r];
-            if (o >= 0) {
-                const int64_t c = o + i - (r > 0 ? int64_t(s_row_end[r - 1]) : 0), j = c >> p.page_shift;
+            if (o < 0) continue;
+            const int64_t c = o + i - (r > 0 ? int64_t(s_row_end[r - 1]) : 0), j = c >> p.page_shift;
+            if (j != page_of) {
                 const int64_t held = (o + page - 1) >> p.page_shift;
                 const int64_t share = r > 0 ? int64_t(s_page_end[r - 1]) : 0;
-                const int32_t id = j < held ? __ldcg(p.table + int64_t(r) * p.max_pages + j) : __ldg(p.free_pages + head + share + j - held);
-                at_pos = int32_t(c);
-                if (id >= 0 && id < p.n_pages) {
-                    slot = int32_t((int64_t(id) << p.page_shift) + (c & (page - 1)));
-                } else if (p.err != nullptr) {
-                    atomicOr(p.err, FNB_ERR_PAGES);
-                }
+                id = j < held ? __ldcg(p.table + int64_t(r) * p.max_pages + j) : __ldg(p.free_pages + head + share + j - held);
+                page_of = j;
+            }
+            at_pos[k] = int32_t(c);
+            if (id >= 0 && id < p.n_pages) {
+                slot[k] = int32_t((int64_t(id) << p.page_shift) + (c & (page - 1)));
+            } else if (p.err != nullptr) {
+                atomicOr(p.err, FNB_ERR_PAGES);
             }
         }
-        p.slots[i] = slot;
-        p.pos[i] = at_pos;
+        auto put = [&](int32_t * to, const int32_t (&v)[ROWS]) {
+            if constexpr (ROWS == 4) {
+                if (i0 + 4 <= p.rows && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+                    *reinterpret_cast<int4 *>(to + i0) = make_int4(v[0], v[1], v[2], v[3]);
+                    return;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k) {
+                if (i0 + k < p.rows) to[i0 + k] = v[k];
+            }
+        };
+        put(p.slots, slot);
+        put(p.pos, at_pos);
     }
 }
 
@@ -206,6 +230,7 @@ extern "C" int32_t fnb_page_tables(const fnb_page_tables_args * a, void * stream
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = unsigned(ctas), attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr, cfg.numAttrs = ctas > 1 ? 2 : 1;
-    (void) cudaLaunchKernelEx(&cfg, page_tables_kernel, p);
+    // four rows at a time once each thread has several: 65 536 rows of 96 requests 10.0 us against 11.5
+    (void) cudaLaunchKernelEx(&cfg, a->rows > int64_t(ctas) * kThreadsT ? page_tables_kernel<4> : page_tables_kernel<1>, p);
     return launch_status();
 }

@@ -67,3 +67,38 @@ def test_more_tiles_than_the_line_counts(dev):
     ops.attend_paged_kv4(q, kc, kc, ks, ks, table, lens, page_size=page, out=out, err=err)
     torch.cuda.synchronize()
     assert int(err.item()) == ops.ERR_PAGES and bool((out == 9.0).all())
+
+
+@pytest.mark.parametrize("rows,shift", [(30, 1), (5000, 0), (20000, 1), (20003, 2), (66001, 3)])
+def test_slot_map_in_arrays_of_any_alignment(dev, rows, shift):
+    """Slots and positions into views that begin anywhere: the same numbers, and nothing beside them."""
+    g = synth.rng(420 + rows)
+    n_req, page = 37, 16
+    old = g.integers(0, 90, n_req).astype(np.int32)
+    new = np.diff(np.concatenate(([0], np.sort(g.integers(0, rows - 4, n_req - 1)), [rows - 5]))).astype(np.int32)
+    held = -(-old // page)
+    n_pages = int((-(-(old + new) // page)).sum()) + 5
+    ids = g.permutation(n_pages).astype(np.int32)
+    table = np.full((n_req, int((-(-(old + new) // page)).max()) + 1), -1, np.int32)
+    at = 0
+    for r in range(n_req):
+        table[r, :held[r]] = ids[at:at + held[r]]
+        at += held[r]
+    want_slot, want_pos = np.full(rows, -1, np.int64), np.full(rows, -1, np.int64)
+    i, free = 0, at
+    for r in range(n_req):
+        need = -(-(old[r] + new[r]) // page) - held[r]
+        pages = np.concatenate((table[r, :held[r]], ids[free:free + need])).astype(np.int64)
+        free += need
+        c = old[r] + np.arange(new[r])
+        want_slot[i:i + new[r]], want_pos[i:i + new[r]] = pages[c // page] * page + c % page, c
+        i += int(new[r])
+    slots, pos = (torch.full((rows + 8,), 77, dtype=torch.int32, device=dev) for _ in range(2))
+    err = ops.new_err(dev)
+    ops.page_tables(to_dev(table, dev), to_dev(old, dev), to_dev(new, dev), to_dev(ids[at:], dev), page_size=page, n_pages=n_pages,
+                    rows=rows, slots=slots[shift:shift + rows], pos=pos[shift:shift + rows], err=err)
+    assert int(err.item()) == 0
+    for got, want in ((slots, want_slot), (pos, want_pos)):
+        got = got.cpu().numpy()
+        assert np.array_equal(got[shift:shift + rows], want)
+        assert (got[:shift] == 77).all() and (got[shift + rows:] == 77).all()
