@@ -59,7 +59,7 @@ constexpr int kMaxReq = 2048;
 constexpr float kLog2eF = 1.4426950408889634f;
 constexpr int kStart = 1;                        // units that an item's start counts
 constexpr int kMaxShare = 8;                     // CTAs that share an item in the clustered form, at most
-constexpr float kPShift = 14.0f;                 // probabilities are held times 2^14
+constexpr float kPShift = 14.0f;                 // a row's weights are held so that the largest is 2^14 (from 2^24 on, 1 to 2^14)
 
 // ---- geometry -------------------------------------------------------------------------------------------------------
 // HD: head_dim.  NT: blocks of eight query columns a unit serves (1, or 2 at 256); 0: four columns, whose large and small
@@ -748,17 +748,22 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
                 float2 v = *reinterpret_cast<const float2 *>(s_wmax + ((it & 1) * 8 + g) * G::kCols + x * 8 + t2);
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) v.x = fmaxf(v.x, __shfl_xor_sync(kFull, v.x, o)), v.y = fmaxf(v.y, __shfl_xor_sync(kFull, v.y, o));
-                const float n0 = fmaxf(mx[x][0], v.x * sc[x][0]), n1 = fmaxf(mx[x][1], v.y * sc[x][1]);
+                // The reference is the maximum less kPShift, rounded up: beside scores past 2^24 the shift is lost in the
+                // rounding, and only upwards does no weight pass 2^kPShift.  Products are rounded here and below alike, so
+                // that the cell of the maximum has exactly the maximum's.  (Two scalar operations a score: a packed product
+                // and a packed sum are compiled into one FMA, rounding modes and -fmad=false notwithstanding, and an FMA leaves
+                // the product unrounded: past 2^25 that gave weights of infinity, or of zero in all cells.)
+                const float n0 = fmaxf(mx[x][0], __fadd_ru(__fmul_rn(v.x, sc[x][0]), -kPShift));
+                const float n1 = fmaxf(mx[x][1], __fadd_ru(__fmul_rn(v.y, sc[x][1]), -kPShift));
                 const float f0 = n0 == -INFINITY ? 0.0f : n0, f1 = n1 == -INFINITY ? 0.0f : n1;
                 r0 = ex2(mx[x][0] - f0), r1 = ex2(mx[x][1] - f1);
                 mx[x][0] = n0, mx[x][1] = n1;
                 ls[x][0] *= r0, ls[x][1] *= r1;
                 if (NT > 1 && wid == 0 && g == 0) *reinterpret_cast<float2 *>(s_corr + (it & 1) * G::kCols + x * 8 + 2 * t) = make_float2(r0, r1);
-                const float b0 = kPShift - f0, b1 = kPShift - f1;
 #pragma unroll
                 for (int s = 0; s < SL; ++s) {
-                    const float e0 = ex2(fmaf(sv[s][x][0], sc[x][0], b0)), e1 = ex2(fmaf(sv[s][x][1], sc[x][1], b1));
-                    const float e2 = ex2(fmaf(sv[s][x][2], sc[x][0], b0)), e3 = ex2(fmaf(sv[s][x][3], sc[x][1], b1));
+                    const float e0 = ex2(__fsub_rn(__fmul_rn(sv[s][x][0], sc[x][0]), f0)), e1 = ex2(__fsub_rn(__fmul_rn(sv[s][x][1], sc[x][1]), f1));
+                    const float e2 = ex2(__fsub_rn(__fmul_rn(sv[s][x][2], sc[x][0]), f0)), e3 = ex2(__fsub_rn(__fmul_rn(sv[s][x][3], sc[x][1]), f1));
                     ls[x][0] += e0 + e2, ls[x][1] += e1 + e3;
                     uint32_t h0, h1, q0, q1;
                     split2(e0, e1, h0, q0);

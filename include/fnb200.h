@@ -464,7 +464,8 @@ int32_t fnb_attend_static(const fnb_attend_args * args, void * stream);
  * n_kv_heads) are served eight to a pass over its cells (four when max_rows gives no more and head_dim is at least 128,
  * sixteen when it gives more than eight and head_dim is 256); more columns are more passes, read mostly from L2.  A wrong hint costs time, not results.
  * F32 softmax statistics; products on the tensor cores with queries and probabilities split into two FP16 parts, cells
- * exact: relative error (2-norm) against a 64-bit evaluation about 5e-7.  |q| below 2^64.
+ * exact: relative error (2-norm) against a 64-bit evaluation about 5e-7, and scores as exact as F32 holds them however large
+ * they are.  |q| below 2^64, and scale times a sum below 2^126: a row with a score past F32's range gives NaN.
  * A page id outside the cache, a length outside [0, max_pages page_size], or a row range outside [0, rows) sets
  * FNB_ERR_PAGES; the rows of that request then mean nothing, others are unaffected.
  * head_dim 64, 128 or 256; n_req in [1, 2048]; page_size a power of two from 16 to 2^20; cache_slots a multiple of it
