@@ -156,10 +156,12 @@ __global__ void __launch_bounds__(kThreads, 1) rope_kv_pipe_kernel(const rope_ke
             const uint32_t ph = uint32_t(it / stages) & 1u;
             const int64_t t0 = tile * tt;
             const int live = int(a.rows - t0 < tt ? a.rows - t0 : tt);
-            // positions and slots do not depend on the stage: fetch them before waiting for it, a token a lane
+            // Positions and slots do not depend on the stage: fetch them before waiting for it, a token a lane.  (Nothing is
+            // computed from them before the copies are on their way: a choice between the two up here held the copies back
+            // for a load's latency, 0.1 us of a small call.)
             const bool mine = lane < live && (lane & (share - 1)) == member;
             const int32_t p_mine = mine ? __ldg(a.pos + t0 + lane) : 0;
-            const int64_t c_mine = mine && a.slots != nullptr ? int64_t(__ldg(a.slots + t0 + lane)) : int64_t(p_mine);
+            const int32_t s_mine = mine && a.slots != nullptr ? __ldg(a.slots + t0 + lane) : 0;
             if (it >= stages && !mbar_wait(&empty[s], ph ^ 1u, a.err)) break;
             uint8_t * st = data + size_t(s) * stage_bytes;
             if (member == 0 && lane == 0) {
@@ -186,7 +188,10 @@ __global__ void __launch_bounds__(kThreads, 1) rope_kv_pipe_kernel(const rope_ke
                     for (int c = 0; c < 32; ++c) theta = __fmul_rn(theta, a.theta_scale);
                 }
             }
-            if (mine) cell_of[s * tt + lane] = rope_slot_ok<F>(c_mine, a.cache_slots, a.err, true) ? int32_t(c_mine) : -1;
+            if (mine) {
+                const int32_t slot = a.slots != nullptr ? s_mine : p_mine;
+                cell_of[s * tt + lane] = rope_slot_ok<F>(slot, a.cache_slots, a.err, true) ? slot : -1;
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[s]);
         }
