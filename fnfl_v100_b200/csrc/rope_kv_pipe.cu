@@ -156,12 +156,15 @@ __global__ void __launch_bounds__(kThreads, 1) rope_kv_pipe_kernel(const rope_ke
             const uint32_t ph = uint32_t(it / stages) & 1u;
             const int64_t t0 = tile * tt;
             const int live = int(a.rows - t0 < tt ? a.rows - t0 : tt);
-            // Positions and slots do not depend on the stage: fetch them before waiting for it, a token a lane.  (Nothing is
-            // computed from them before the copies are on their way: a choice between the two up here held the copies back
-            // for a load's latency, 0.1 us of a small call.)
+            // positions and slots do not depend on the stage: fetch them before waiting for it, a token a lane
             const bool mine = lane < live && (lane & (share - 1)) == member;
-            const int32_t p_mine = mine ? __ldg(a.pos + t0 + lane) : 0;
+            int32_t p_mine = mine ? __ldg(a.pos + t0 + lane) : 0;
             const int32_t s_mine = mine && a.slots != nullptr ? __ldg(a.slots + t0 + lane) : 0;
+            // The ring's first copies go out at once: nothing is computed from the positions before (held back for their
+            // latency, a small call takes 0.1 us more).  Later copies wait for them, which this exchange of a lane with
+            // itself makes sure of: copies that follow one another faster than that, in rings that are full anyway, cost
+            // large launches 8 % (32 768 tokens of 16 + 2 + 2 heads of 256 into Q8_0: 196 us against 212).
+            if (it >= stages) p_mine = __shfl_sync(kFull, p_mine, lane);
             if (it >= stages && !mbar_wait(&empty[s], ph ^ 1u, a.err)) break;
             uint8_t * st = data + size_t(s) * stage_bytes;
             if (member == 0 && lane == 0) {
