@@ -432,12 +432,18 @@ bool launch_one(const rope_kernel_args & a, cudaStream_t s) {
     const size_t smem = need(tt, stages);
 
     if (!ensure_configured<HD, F>()) return false;
-    // A token's angles are ~2500 cycles of dependent FP64 operations in one warp; the traffic of a token of 30 KB takes
-    // half of that.  Two warps keep up with such tokens (and more copies under way at once cost the 38 KB ones 6 %: 404
-    // against 428 us at 65 536 tokens of 16 + 2 + 2 heads of 256), four with smaller ones (8261 tokens of 8 + 8 + 8 heads of
-    // 128: 75 us with two, 36 with four).  Tiles of one token have nothing to share.
+    // A token's angles are dependent FP64 operations in one warp: about 1.25 us and 0.2 more for every 32 pairs; its traffic
+    // takes an SM 0.68 us for 30 KB.  Two warps keep up with such tokens (and more copies under way at once cost the 38 KB
+    // ones 6 %: 404 against 428 us at 65 536 tokens of 16 + 2 + 2 heads of 256), four with smaller ones (8261 tokens of
+    // 8 + 8 + 8 heads of 128: 75 us with two, 36 with four).  Tiles of one token have nothing to share, and where a token's
+    // traffic takes longer than its angles one warp does (8192 tokens of 32 + 4 + 4 heads of 256: 98 us, with two 113; of
+    // 32 + 2 + 2 without rotation 102 and 107), unless the launch's tensors lie in L2 and the ring is deep (1000 tokens of
+    // 64 + 8 + 8 heads of 128: 13.7 us, with two 10.7; 128 + 8 + 8, a ring of two: 23.2 and 26.2).
     const int64_t token = int64_t(2 * a.n_q + 2 * a.n_kv) * HD * 4;
-    const int share = tt > 1 ? 2 : 1, warps = token >= 30000 ? 2 : kProducerWarps;
+    const float angles = a.n_rot > 0 ? 1.25f + 0.2f * float((a.n_rot / 2 + 31) / 32) : 0.0f, traffic = float(token) * 0.68f / 30000.0f;
+    const bool near = token * a.rows <= 100 * 1000000 && stages == 4 && a.n_rot > 0;
+    const int share = tt > 1 ? 2 : 1;
+    const int warps = token < 30000 ? kProducerWarps : tt == 1 && traffic >= angles && !near ? 1 : 2;
     const int crews = warps / share < stages ? warps / share : stages;
     const int64_t n_tiles = (a.rows + tt - 1) / tt;
     const int grid = int(n_tiles < kSmCount ? n_tiles : kSmCount);
