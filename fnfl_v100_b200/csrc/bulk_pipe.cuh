@@ -74,6 +74,15 @@ __device__ __forceinline__ bool mbar_wait(uint64_t * bar, uint32_t parity, uint3
     if (err != nullptr) atomicOr(err, FNB_ERR_TIMEOUT);
     return false;
 }
+// A build with a limit of a few polls holds a producer's first copies back for some 100 us: where consumers set up a table
+// before they first look, the only tile of a small launch may have landed by then, and whether a wait runs out would be a
+// matter of chance.  Nothing in the product.
+__device__ __forceinline__ void hold_back_producer() {
+    if constexpr (kPrimarySpinLimit < 1024u) {
+        const long long from = clock64();
+        for (int i = 0; i < 100000 && clock64() - from < 200000; ++i) __nanosleep(64);
+    }
+}
 // the unwinding wait: the producer's last look at a stage it has issued a copy into (always the full limit)
 __device__ __forceinline__ bool mbar_wait_landed(uint64_t * bar, uint32_t parity) {
     for (uint32_t i = 0; i < kSpinLimit; ++i) {

@@ -121,6 +121,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (wid == kConsumerWarps) {
         // ---------------- producer: one lane streams the tiles ----------------
         if (lane != 0) return;
+        hold_back_producer();
         const uint64_t policy = l2_evict_first_policy();
         int it = 0;
         bool ok = true;
