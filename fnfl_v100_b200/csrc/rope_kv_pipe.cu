@@ -38,17 +38,11 @@ namespace {
 #ifndef FNB_ROPE_GROUP_WARPS
 #define FNB_ROPE_GROUP_WARPS 10
 #endif
-#ifndef FNB_ROPE_PRODUCERS
-#define FNB_ROPE_PRODUCERS 4
-#endif
-#ifndef FNB_ROPE_MAX_STAGES
-#define FNB_ROPE_MAX_STAGES 4
-#endif
-static_assert(FNB_ROPE_PRODUCERS == 4 && FNB_ROPE_MAX_STAGES == 4, "crews divide the stages evenly");
 constexpr int kGroups = FNB_ROPE_GROUPS;
 constexpr int kGroupWarps = FNB_ROPE_GROUP_WARPS;
 constexpr int kConsumerWarps = kGroups * kGroupWarps;
-constexpr int kProducerWarps = FNB_ROPE_PRODUCERS;
+constexpr int kProducerWarps = 4;  // at most
+constexpr int kMaxStages = 4;
 constexpr int kThreads = (kConsumerWarps + kProducerWarps) * 32;
 constexpr int kSlotBytes = 288;    // a 272-byte cell, padded to 16
 constexpr int kMaxTile = 8;        // tokens per tile at most
@@ -413,7 +407,7 @@ bool launch_one(const rope_kernel_args & a, cudaStream_t s) {
     };
     // the ring: a multiple of the group count (a stage always goes to the same group), as deep as the budget allows
     auto fit = [&](int t) {
-        int st = (FNB_ROPE_MAX_STAGES / kGroups) * kGroups;
+        int st = (kMaxStages / kGroups) * kGroups;
         while (st >= kGroups && need(t, st) > kSmemBudget) st -= kGroups;
         return st;
     };
@@ -444,7 +438,8 @@ bool launch_one(const rope_kernel_args & a, cudaStream_t s) {
     const bool near = token * a.rows <= 100 * 1000000 && stages == 4 && a.n_rot > 0;
     const int share = tt > 1 ? 2 : 1;
     const int warps = token < 30000 ? kProducerWarps : tt == 1 && traffic >= angles && !near ? 1 : 2;
-    const int crews = warps / share < stages ? warps / share : stages;
+    int crews = warps / share < stages ? warps / share : stages;
+    while (stages % crews != 0) crews /= 2;   // a stage belongs to one crew, whatever the number of groups leaves for a ring
     const int64_t n_tiles = (a.rows + tt - 1) / tt;
     const int grid = int(n_tiles < kSmCount ? n_tiles : kSmCount);
     const pipe_shape sh{tt, stages, nbh, uint32_t((0x100000000ull + uint64_t(rpt) - 1) / uint64_t(rpt)), share, crews};
