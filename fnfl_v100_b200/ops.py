@@ -80,6 +80,13 @@ def _numel(t: torch.Tensor | None, n: int, name: str) -> None:
         raise ValueError(f"{name}: expected {n} elements, got {t.numel()}")
 
 
+def _int32(v: int, name: str) -> int:
+    """`v`, refused where the C structure would keep its low 32 bits only."""
+    if not -2**31 <= v < 2**31:
+        raise ValueError(f"{name}: {v} does not fit 32 bits")
+    return v
+
+
 def _err(err: torch.Tensor | None) -> torch.Tensor | None:
     if err is not None:
         _dev(err, torch.int32, "err")
@@ -277,7 +284,7 @@ def _rope_args(q, k, v, pos, slots, q_norm_w, k_norm_w, q_out, k_cache, v_cache,
     cache_slots = k_cache.shape[0]
     a = _lib.RopeKvArgs(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), _at(slots), _at(q_norm_w), _at(k_norm_w), q_out.data_ptr(),
-        k_cache.data_ptr(), v_cache.data_ptr(), _at(k_f32), _at(err), rows, cache_slots, n_q, k.shape[1], hd, n_rot, ts, eps,
+        k_cache.data_ptr(), v_cache.data_ptr(), _at(k_f32), _at(err), rows, cache_slots, n_q, k.shape[1], hd, _int32(n_rot, "n_rot"), ts, eps,
         _at(planes))
     return a
 
@@ -337,6 +344,8 @@ def page_tables(table: torch.Tensor, n_old: torch.Tensor, n_new: torch.Tensor, f
     if table.dim() != 2:
         raise ValueError("table: expected [n_req][max_pages]")
     n_req, max_pages = table.shape
+    if not 1 <= rows < 2**31:
+        raise ValueError("rows: expected 1 to 2^31 - 1")
     for name, t in (("n_old", n_old), ("n_new", n_new)):
         _numel(_dev(t, torch.int32, name), n_req, name)
     _dev(free_pages, torch.int32, "free_pages")
@@ -348,13 +357,14 @@ def page_tables(table: torch.Tensor, n_old: torch.Tensor, n_new: torch.Tensor, f
         if outs[i] is not None:
             _numel(_dev(outs[i], torch.int32, name), sizes[i], name)
     with _on(table, n_old, n_new, free_pages, free_head, slots, pos, row_start, n_cells, free_head_out, _err(err)):
-        if rows > 0 and outs == [None] * 5:   # one allocation for all of them
+        if outs == [None] * 5:   # one allocation for all of them
             outs = table.new_empty(2 * rows + 2 * n_req + 2).split_with_sizes(sizes)
         else:
             outs = [table.new_empty(n) if t is None else t for t, n in zip(outs, sizes)]
         a = _lib.PageTablesArgs(n_old.data_ptr(), n_new.data_ptr(), free_pages.data_ptr(), _at(free_head), table.data_ptr(),
                                 outs[3].data_ptr(), outs[2].data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(), outs[4].data_ptr(),
-                                _at(err), rows, free_pages.numel(), n_req, max_pages, n_pages, page_size)
+                                _at(err), rows, free_pages.numel(), n_req, max_pages, _int32(n_pages, "n_pages"),
+                                _int32(page_size, "page_size"))
         _check(_lib.lib().fnb_page_tables(C.byref(a), _raw_stream(table)), "page_tables")
     return PageTables(*outs)
 
@@ -402,6 +412,8 @@ def kv4_read_f32(cache: torch.Tensor, scale: torch.Tensor, *, cells: torch.Tenso
         rows = _dev(cells, torch.int32, "cells").numel()
     elif rows is None:
         rows = slots - cell0
+    if rows < 1 or (cells is None and not 0 <= cell0 <= slots - rows):
+        raise ValueError("cells / cell0 / rows: expected at least one row, within the cache")
     with _on(cache, scale, cells, out, _err(err)):
         if out is None:
             out = cache.new_empty((rows, n_kv, hd), dtype=torch.float32)
@@ -449,7 +461,7 @@ def attend_paged_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
             _numel(_dev(out, torch.float32, "out"), q.numel(), "out")
         a = _lib.AttendPagedArgs(q.data_ptr(), _at(gate), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                  table.data_ptr(), n_cells.data_ptr(), _at(row_start), out.data_ptr(), None, 0, _at(err), slots,
-                                 q.shape[0], n_req, max_pages, page_size, max_rows, q.shape[1], n_kv, hd,
+                                 q.shape[0], n_req, max_pages, _int32(page_size, "page_size"), _int32(max_rows, "max_rows"), q.shape[1], n_kv, hd,
                                  hd ** -0.5 if scale is None else float(scale), stride)
         need = _lib.lib().fnb_attend_paged_workspace_bytes(C.byref(a))
         if need == 0:
