@@ -25,7 +25,9 @@
 //
 // Work split: a unit is a tile of 128 cells (256 of narrow heads) of one (request, KV head, block of query columns), an
 // item, or an item's start: its queries, first copies and last sums cost about what a tile does, and a line of tiles alone
-// left the pieces with most items behind (64 requests of up to 8192 cells 64.7 us against 59.9; two units a start 62.2).
+// left the pieces with most items behind.  With none, one and two units a start: 64 requests of up to 8192 cells 68.4, 64.1 and
+// 64.0 us, 40 of up to 5000 with 32 heads over 8 of 128 51.3, 44.0 and 46.1, 13 of up to five rows 57.0, 54.1 and 55.5.  What it
+// costs: a lone request whose tiles divide evenly among the CTAs gives some of them one more (18 944 cells 11.9, 14.8 and 14.9).
 // The units of all requests form one line that is cut into equal pieces, one for each resident CTA, wherever the requests'
 // borders fall: one long request and many ragged ones both fill the machine, from lengths only the device knows.  A piece
 // that holds all tiles of an item writes its rows itself; otherwise it leaves its sums, maximum and accumulators in the
@@ -43,9 +45,11 @@
 // scheduler.  The change took 61 us to 50 at 196 608 cells.)
 //
 // Measured on a B200, graph replays over caches larger than L2: one request of 196 608 cells, 16 heads over 2 of 256:
-// 43.2 us, 113 MB at 2.6 TB/s; 40 requests of up to 5000 cells, 32 heads over 8 of 128: 43 us; 8 requests of up to 300
-// cells: 7.5 us, latency.  In its steady state a warp issues some 790 instructions a tile at 0.56 to 0.6 an issue slot,
-// the logic, FP16 and tensor units each 35 to 40 % busy; cells that lie in L2 give the same time.
+// 44 us, 113 MB at 2.6 TB/s; 40 requests of up to 5000 cells, 32 heads over 8 of 128: 44 us; 64 of up to 8192, 32 over 8 of 64:
+// 77 us; 8 requests of up to 300 cells: 7.6 us, latency.  A warp issues some 790 instructions a tile, and issue slots are in
+// use 55 to 63 % of the time, logic 35 to 43, tensor 16 to 38: no unit is at its limit, what is waited for is mostly results of the
+// warp's own last instructions (1.1 to 2.4 warps an issue) with four warps a scheduler to hide them.  Cells that lie in L2 give
+// the same time.
 #include <atomic>
 #include <type_traits>
 
@@ -1028,8 +1032,8 @@ attend_paged_kernel(const __grid_constant__ paged_params p) {
 // and sums joined in the order of the pieces.  LISTED: block k takes the k-th, (k + gridDim.x)-th .. of the cut items,
 // found by listing the pieces' marks (few items, each in many pieces: few blocks an item would leave most of the machine
 // idle); all weights are made first, from maxima in shared memory.  Else block k looks at piece k + 1 alone, which costs one
-// load where there is nothing to fold, and as its items lie in few pieces each thread joins its own as they arrive (40
-// requests of up to 5000 cells, 320 items: 43.1 us against 44.9; items in ten pieces or more lose 1 to 2 us that way).
+// load where there is nothing to fold, and as its items lie in few pieces each thread joins its own as they arrive (when it
+// was added, 40 requests of up to 5000 cells, 320 items: 43.1 us against 44.9; items in ten pieces or more lost 1 to 2 us).
 constexpr int kFoldThreads = 256;
 constexpr int kMaxPieces = 2 * kSmCount;
 template <int HD, int COLS, int VEC, bool LISTED>
@@ -1257,10 +1261,11 @@ int64_t expected_items(const fnb_attend_paged_args * a, const paged_params & p) 
     return int64_t(a->n_req) * a->n_kv_heads * blocks;
 }
 // The shared form: short items, few enough that each can have a cluster at once.  As many CTAs as tiles where the grid
-// allows it, else the most that leave a CTA two tiles; items that are longer or more numerous go on the line.  Nothing is
-// left in memory and the second launch falls away (16 heads over 2 of 256, us, line against shared: 8 requests of up to 300
-// cells 10.4 and 8.1, 64 of up to 500 18.9 and 12.3, one of 1000 9.4 and 7.1, 16 of 2000 12.6 and 11.9; but 64 of 1000, four
-// tiles a CTA, 20.5 and 22).  Returns log2 of the CTAs, 0 for the line.
+// allows it (two for one tile), else the most that leave a CTA two tiles; items that are longer or more numerous go on the line.
+// Nothing is left in memory and the second launch falls away (16 heads over 2 of 256, us, line against shared: 8 requests of up
+// to 300 cells 10.5 and 7.6, 64 of up to 500 18.4 and 12.6, one of 1000 9.6 and 7.7, 16 of 2000 14.3 and 12.4; but 64 of 1000, four
+// tiles a CTA, 20.5 and 22).  A lone tile gains too, against an item a CTA takes whole: the walk is shorter (one request of
+// 128 cells 6.0 and 5.5, 70 of them 8.5 and 7.4).  Returns log2 of the CTAs, 0 for the line.
 template <int HD, int NT>
 int share_of(const paged_params & p, int64_t items) {
     const int64_t tiles = (p.cells_max + geo<HD, NT>::kTile - 1) / geo<HD, NT>::kTile;
@@ -1316,7 +1321,10 @@ int32_t launch_paged(const fnb_attend_paged_args * a, paged_params & p, cudaStre
     launch_pdl(attend_paged_kernel<HD, NT, false>, grid, geo<HD, NT>::kThreads, geo<HD, NT>::total, s, p);
     if (cudaPeekAtLastError() != cudaSuccess) return FNB_LAUNCH_FAILED;
     if (fold) {
-        // Few items of a long table: list them.
+        // Few items: list them, and where each may lie in 64 pieces or more, a block takes 32 dims instead of a whole head
+        // (one request, 16 heads over 2 of 256, by 32 dims, by heads, unlisted: 4096 cells 11.0, 10.9 and 10.8 us, 8192 12.0,
+        // 13.9 and 14.7, 196 608 43.7, 46.9 and 56.6; 20 requests of up to 4096, where the blocks are more than run at a time, 29.0,
+        // 19.6 and 19.1).  Unlisted from a wave of columns on (40 requests of 32 over 8 heads of 128: 49.1 listed, 44.0).
         const int64_t outputs = items * int64_t(cols), wave = kSmCount * 8;   // columns to fold; blocks that run at a time
         if (outputs * (HD / 32) <= wave && p.cells_max >= 64 * 128) {
             launch_fold(attend_paged_fold_kernel<HD, kCols, 8, true>, dim3(unsigned(items), unsigned(cols), HD / 32), s, p, grid);

@@ -113,9 +113,12 @@ __device__ __forceinline__ int group_sum(int v) {
 // ---- the scalar rules of the 8-bit block formats ---------------------------------------------------------
 // four int32 codes -> four packed int8 (low byte of each), and the sum of four packed int8
 // ---- two FP32 operations per instruction (fma / mul / add .f32x2 of sm_100) ---------------------------------
-// Each half of the pair is the IEEE round-to-nearest operation, so results are the scalar ones.  For kernels bound by
-// instruction issue rather than by the FP32 pipe (SwiGLU: the written-out division is seven dependent FP32 operations
-// per value) this halves those instructions.
+// Each half of the pair is the IEEE round-to-nearest operation, so results are the scalar ones - unless a packed product goes
+// into a packed sum and nowhere else: the compiler makes one FMA of the two, with one rounding, -fmad=false and the .rn of
+// both notwithstanding (seen in every one of 65 536 pairs).  Where both roundings count, one of the two stays scalar, or the
+// product has a second use, as in ggml_q8_rule::code4 (its codes are the scalar rule's over 4.5e9 values at the codes' borders).
+// For kernels bound by instruction issue rather than by the FP32 pipe (SwiGLU: the written-out division is seven dependent
+// FP32 operations per value) this halves those instructions.
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pk(float x, float y) {
     f32x2 r;

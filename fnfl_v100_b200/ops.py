@@ -384,7 +384,8 @@ def rope_neox_kv4_append(q, k, v, pos, *, n_rot: int, theta_scale: float, k_cach
                          slots=None, q_norm_w=None, k_norm_w=None, eps: float = 1e-6, q_out=None, k_f32=None,
                          err=None, planes=None):
     """The norm + RoPE + append step into KV4 planes (new_kv_cache(fmt="kv4")): groups of 32 values as 4-bit codes and an
-    FP16 scale.  A slot of -1 is a row of padding, for which nothing is written.  Returns q_out."""
+    FP16 scale.  A slot of -1 is a row of padding, for which nothing is written: its rows of q_out (and k_f32) stay as they were,
+    uninitialised where q_out is allocated here.  Returns q_out."""
     n_kv, n_slots, hd = _kv4_planes(k_cache, k_scale, "k")
     if _kv4_planes(v_cache, v_scale, "v") != (n_kv, n_slots, hd) or k.shape[1:] != (n_kv, hd):
         raise ValueError("k_cache / v_cache: expected the planes of new_kv_cache for these heads")
@@ -406,7 +407,8 @@ def rope_neox_kv4_append(q, k, v, pos, *, n_rot: int, theta_scale: float, k_cach
 
 def kv4_read_f32(cache: torch.Tensor, scale: torch.Tensor, *, cells: torch.Tensor | None = None, cell0: int = 0,
                  rows: int | None = None, out: torch.Tensor | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
-    """Rows of a KV4 plane widened to F32: out [rows][n_kv][head_dim] = the values of slots cells[t] (int32), or cell0 + t."""
+    """Rows of a KV4 plane widened to F32: out [rows][n_kv][head_dim] = the values of slots cells[t] (int32), or cell0 + t.  The
+    row of a slot of -1 (padding) or outside the cache (ERR_SLOT) is not written: uninitialised where out is allocated here."""
     n_kv, slots, hd = _kv4_planes(cache, scale, "kv")
     if cells is not None:
         rows = _dev(cells, torch.int32, "cells").numel()
@@ -434,8 +436,8 @@ def attend_paged_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     """Attention of q [rows][n_q][hd] over the paged KV4 cache: request r's rows are row_start[r] .. row_start[r + 1] - 1 (None:
     one row a request) and see its n_cells[r] cells, the pages table[r] lists, causally.  max_rows: the most rows of a request
     (a hint).  `table` may be the first columns of a wider one (table[:, :w], once no request has more pages): narrow tables are
-    served faster.  Rows of no request are left as they were in `out`, which may not overlap an input.  `workspace` (uint8) is used
-    when it is large enough, else one is allocated.  Returns out [rows][n_q][hd]."""
+    served faster.  Rows of no request are left as they were in `out` (uninitialised where it is allocated here), which may not
+    overlap an input.  `workspace` (uint8) is used when it is large enough, else one is allocated.  Returns out [rows][n_q][hd]."""
     _dev(q, torch.float32, "q")
     n_kv, slots, hd = _kv4_planes(k_cache, k_scale, "k")
     if q.dim() != 3 or q.shape[2] != hd or _kv4_planes(v_cache, v_scale, "v") != (n_kv, slots, hd):

@@ -38,8 +38,9 @@ extern "C" {
                               fn/kernels/qsa/attend.cu:264-281); the launch's outputs are incomplete */
 
 #define FNB_ERR_PAGES 8u   /* fnb_page_tables: a request whose rows or pages do not fit, or a page id outside the cache;
-                              fnb_attend_paged_kv4: a page id outside the cache.  No counterpart in the reference,
-                              whose cache is one dense range */
+                              fnb_attend_paged_kv4: a page id outside the cache, a length or a range of rows outside its
+                              bounds, or more tiles than the call can count.  No counterpart in the reference, whose
+                              cache is one dense range */
 
 #define FNB_Q8_0_BLOCK_BYTES 34
 #define FNB_Q8_1_BLOCK_BYTES 36
@@ -462,7 +463,9 @@ int32_t fnb_attend_static(const fnb_attend_args * args, void * stream);
  * give the first columns of one, max_pages of them in rows table_stride apart, once no request is longer.
  * max_rows (a hint; 0 means 1): the most rows a request has.  The query columns of a KV head (rows x n_q_heads /
  * n_kv_heads) are served eight to a pass over its cells (four when max_rows gives no more and head_dim is at least 128,
- * sixteen when it gives more than eight and head_dim is 256); more columns are more passes, read mostly from L2.  A wrong hint costs time, not results.
+ * sixteen when it gives more than eight and head_dim is 256); more columns are more passes, read mostly from L2.  Every pass
+ * visits all cells of the request, those that a prompt's rows do not see yet too, so a long prompt is right but slow: time goes with
+ * passes x cells (1024 rows over 16 384 cells, 16 heads over 2 of 256: 2.2 ms).  A wrong hint costs time, not results.
  * F32 softmax statistics; products on the tensor cores with queries and probabilities split into two FP16 parts, cells
  * exact: relative error (2-norm) against a 64-bit evaluation about 5e-7, and scores as exact as F32 holds them however large
  * they are.  |q| below 2^64, and scale times a sum below 2^126: a row with a score past F32's range gives NaN.
