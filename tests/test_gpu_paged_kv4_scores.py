@@ -83,3 +83,21 @@ def test_one_cell_leads(dev, q_scale, lens, cells, hd, n_q, n_kv, m):
     assert (off <= 2.0**-20 * np.abs(best[clear])).all()
     room = 2.0**-18 * np.maximum(np.abs(low), np.abs(high))
     assert ((got >= low - room) & (got <= high + room)).all()
+
+
+@pytest.mark.parametrize("hd,n_q,n_kv,m", SHAPES)
+@pytest.mark.parametrize("lens,cells", FORMS)
+def test_a_query_that_is_no_number_stays_alone(dev, lens, cells, hd, n_q, n_kv, m):
+    """One head's query holds an infinity or a NaN: that head's row is NaN, every other row and head keeps its bits."""
+    planes, table, q, _, page = large_case(lens, cells, hd, n_q, n_kv, m, 1.0, dev)
+    start = to_dev((np.arange(len(lens) + 1) * m).astype(np.int32), dev)
+    rest = (*planes, to_dev(table, dev), to_dev(np.array(lens, np.int32), dev))
+    call = lambda x: ops.attend_paged_kv4(to_dev(x, dev), *rest, page_size=page, row_start=start, max_rows=m).cpu().numpy()  # noqa: E731
+    clean = call(q)
+    for row, head, what in ((0, 0, np.nan), (0, n_q - 1, np.inf), (len(lens) * m - 1 - 2 * m, 1, -np.inf), (m, 2, np.nan)):
+        x = q.copy()
+        x[row, head, 17] = what
+        got, same = call(x), np.ones(q.shape[:2], bool)
+        same[row, head] = False
+        assert np.array_equal(got[same], clean[same])
+        assert np.isnan(got[row, head]).all() or lens[row // m] - m + row % m + 1 < 1
