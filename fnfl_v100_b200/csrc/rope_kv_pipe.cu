@@ -6,7 +6,7 @@
 // its speed is how many bytes each SM keeps in flight and how few instructions a row costs.  With loads into
 // registers the first is tied to occupancy; with cp.async.bulk it is a shared-memory budget:
 //
-//   producer warps (2 or 4)  one crew of two that share a tile's tokens, or several crews that take tiles in turn.  Per
+//   producer warps (1, 2 or 4)  crews of one, or of two that share a tile's tokens; several crews take tiles in turn.  Per
 //                       tile of `tt` tokens: three bulk copies (the tile's Q, K and V rows are each one contiguous run in
 //                       HBM) into stage s, completion counted in bytes on full[s]; while they fly the tile's producers
 //                       compute its (cos, sin) pairs - the F32 angle chain pos * ts^i and the exact sincos, a token per
